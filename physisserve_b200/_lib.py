@@ -1,5 +1,4 @@
-"""ctypes binding of ``libphysis_b200.so`` (declared in ``include/physis_b200.h`` and
-``include/physis_b200_ltx.h``).
+"""ctypes binding of ``libphysis_b200.so`` (declared in the headers under ``include/``).
 
 The library is loaded from ``physisserve_b200/lib/`` only.  There is no fallback:
 if the shared library is missing, importing the ops raises, so a GPU host can never
@@ -34,6 +33,10 @@ ROPE_SPLIT, ROPE_INTERLEAVED = 0, 1
 LAUNCH_STREAM, LAUNCH_PDL, LAUNCH_PDL_EARLY_INPUTS = 0, 1, 2
 # ps_seq_kind
 SEQ_PREP, SEQ_SINK = 0, 1
+# ps_kv4_kernel
+KV4_AUTO, KV4_ROWS, KV4_TILES = 0, 1, 2
+# PS_KV4_ROW_BYTES
+KV4_ROW_BYTES = 72
 # PS_ATTN_STATIC_SCRATCH_BYTES (include/physis_b200_attention.h)
 ATTN_STATIC_SCRATCH_BYTES = 32 << 20
 
@@ -41,7 +44,9 @@ EXPORTS = ("ps_abi_version", "ps_error_message", "ps_qk_prep_validate", "ps_qk_n
            "ps_device_timeouts", "ps_wait_selftest", "ps_rope", "ps_rope_validate",
            "ps_table_prep_validate", "ps_qk_norm_rope_tables", "ps_rope_tables", "ps_rope_tables_validate",
            "ps_attention_workspace", "ps_attention_validate", "ps_ring_attention", "ps_attention_timeouts",
-           "ps_ring_attention_static")
+           "ps_ring_attention_static",
+           "ps_qk_norm_rope_kv4", "ps_kv4_prep_validate", "ps_kv4_read", "ps_kv4_read_validate", "ps_attention_kv4",
+           "ps_kv4_attention_validate", "ps_kv4_attention_workspace", "ps_kv4_counters")
 
 
 class PsSeq(ctypes.Structure):
@@ -163,6 +168,91 @@ class PsAttnArgs(ctypes.Structure):
     ]
 
 
+class PsKv4Cache(ctypes.Structure):
+    """``ps_kv4_cache`` (include/physis_b200_kv4.h)."""
+
+    _fields_ = [
+        ("pages", ctypes.c_void_p),
+        ("table", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int64),
+        ("members", ctypes.c_int64),
+        ("table_pages", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int32),
+        ("page_rows", ctypes.c_int32),
+        ("k_scale", ctypes.c_float),
+        ("v_scale", ctypes.c_float),
+    ]
+
+
+class PsKv4PrepArgs(ctypes.Structure):
+    """``ps_kv4_prep_args`` (include/physis_b200_kv4.h)."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("table_mode", ctypes.c_int32),
+        ("t_dim", ctypes.c_int32),
+        ("h_dim", ctypes.c_int32),
+        ("w_dim", ctypes.c_int32),
+        ("n_seqs", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("weight_f32", ctypes.c_int32),
+        ("launch", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("in_rows", ctypes.c_int64),
+        ("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64),
+        ("k", ctypes.c_void_p), ("k_stride", ctypes.c_int64),
+        ("v", ctypes.c_void_p), ("v_stride", ctypes.c_int64),
+        ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
+        ("cos", ctypes.c_void_p),
+        ("sin", ctypes.c_void_p),
+        ("table_rows", ctypes.c_int64),
+        ("q_out", ctypes.c_void_p), ("q_out_stride", ctypes.c_int64),
+        ("k_pre", ctypes.c_void_p), ("k_pre_stride", ctypes.c_int64),
+        ("k_sink", ctypes.c_void_p), ("k_sink_stride", ctypes.c_int64),
+        ("k_sink_rows", ctypes.c_int64),
+        ("cache", PsKv4Cache),
+        ("seqs", ctypes.c_void_p),
+    ]
+
+
+class PsKv4ReadArgs(ctypes.Structure):
+    """``ps_kv4_read_args`` (include/physis_b200_kv4.h)."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("row0", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+        ("k_out", ctypes.c_void_p), ("k_member_stride", ctypes.c_int64), ("k_row_stride", ctypes.c_int64),
+        ("v_out", ctypes.c_void_p), ("v_member_stride", ctypes.c_int64), ("v_row_stride", ctypes.c_int64),
+        ("cache", PsKv4Cache),
+    ]
+
+
+class PsKv4AttnArgs(ctypes.Structure):
+    """``ps_kv4_attn_args`` (include/physis_b200_kv4.h)."""
+
+    _fields_ = [
+        ("heads", ctypes.c_int32),
+        ("q_tokens", ctypes.c_int32),
+        ("kv_tokens", ctypes.c_int32),
+        ("causal_block", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("kernel", ctypes.c_int32),
+        ("key_chunks", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("q", ctypes.c_void_p), ("q_member_stride", ctypes.c_int64), ("q_row_stride", ctypes.c_int64),
+        ("out", ctypes.c_void_p), ("out_member_stride", ctypes.c_int64), ("out_row_stride", ctypes.c_int64),
+        ("kv_lens", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("cache", PsKv4Cache),
+    ]
+
+
 _LIB = None
 
 
@@ -213,6 +303,16 @@ def load() -> ctypes.CDLL:
     lib.ps_ring_attention_static.argtypes = [ctypes.c_void_p, ctypes.c_void_p]  # (const ps_attn_args*, stream)
     lib.ps_attention_timeouts.restype = ctypes.c_int32
     lib.ps_attention_timeouts.argtypes = [ctypes.POINTER(ctypes.c_uint32), ctypes.c_int32]
+    for name in ("ps_kv4_prep_validate", "ps_kv4_read_validate", "ps_kv4_attention_validate"):
+        getattr(lib, name).restype = ctypes.c_int32
+        getattr(lib, name).argtypes = [ctypes.c_void_p]
+    for name in ("ps_qk_norm_rope_kv4", "ps_kv4_read", "ps_attention_kv4"):
+        getattr(lib, name).restype = ctypes.c_int32
+        getattr(lib, name).argtypes = [ctypes.c_void_p, ctypes.c_void_p]  # (const args*, stream)
+    lib.ps_kv4_attention_workspace.restype = ctypes.c_int32
+    lib.ps_kv4_attention_workspace.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_int64)]
+    lib.ps_kv4_counters.restype = ctypes.c_int32
+    lib.ps_kv4_counters.argtypes = [ctypes.POINTER(ctypes.c_uint32), ctypes.c_int32]
     version = lib.ps_abi_version()
     if version != ABI_VERSION:
         raise ImportError(f"{LIB_PATH} has ABI version {version}, expected {ABI_VERSION}")

@@ -1,0 +1,683 @@
+// Attention over the paged 4-bit K/V cache (include/physis_b200_kv4.h), sm_100a.
+//
+// A K/V head's query rows are its (token, query head) pairs: row r = t * group + i is token t of
+// query head kv_head * group + i, so query heads that share a K/V head share every byte read.
+
+#include <math.h>
+#include <stdio.h>
+#include <string.h>
+
+#include <mutex>
+
+#include "ps_kv4.cuh"
+#include "ps_sm100.cuh"
+
+namespace ps {
+namespace {
+
+constexpr int kTileKeys = 128;  // keys per tile: one page of the largest size
+constexpr int kMaxChunks = 64;
+constexpr int kTileBytes = kTileKeys * 2 * kKv4Row;
+
+struct AParams {
+  Kv4Dev cache;
+  const __nv_bfloat16* q;
+  __nv_bfloat16* out;
+  const int32_t* lens;
+  int64_t q_member, q_row, out_member, out_row;
+  int32_t Lq, kv_max, causal_block, group;
+  int32_t rows;          // query rows of a K/V head: Lq * group
+  int32_t row_blocks;    // blocks of query rows per K/V head
+  int32_t chunks;        // key chunks per unit
+  int32_t grid;          // persistent CTAs (tiles kernel)
+  int64_t units;         // members * kv_heads * row_blocks
+  float scale_log2;      // softmax scale * k_scale * log2(e)
+  float* ws_o;           // [units][chunks][rows of a block][128] unnormalised sums (chunks > 1)
+  float2* ws_ml;         // [units][chunks][rows of a block] (reference in log2 units, sum)
+};
+
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int* abort_flag, bool count = true) {
+  return bar_wait_for(bar, parity, abort_flag, count, &g_kv4_counts[kKv4Timeouts]);
+}
+
+// The warp's wait: a test that does not block first (the phase has often completed already).
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int lane) {
+  if (__all_sync(0xffffffffu, bar_test(bar, parity))) return true;
+  return __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag, lane == 0));
+}
+
+// Window rows of member b.
+__device__ __forceinline__ int member_len(const AParams& p, int b) {
+  if (!p.lens) return p.kv_max;
+  const int n = p.lens[b];
+  return n < 0 ? 0 : (n > p.kv_max ? p.kv_max : n);
+}
+// Keys that token t of a member with n window rows sees.
+__device__ __forceinline__ int token_limit(const AParams& p, int n, int t) {
+  if (p.causal_block == 0) return n;
+  const int64_t lim = static_cast<int64_t>(n) - p.Lq + static_cast<int64_t>(t / p.causal_block + 1) * p.causal_block;
+  return lim < 0 ? 0 : (lim > n ? n : static_cast<int>(lim));
+}
+
+// Power of two that brings a row's largest magnitude `top` (>= 0) into [1, 2), and its inverse; 1 for
+// zero, subnormal and non-finite rows.
+__device__ __forceinline__ float row_power(float top, float& back) {
+  const uint32_t e = __float_as_uint(top) >> 23;
+  if (e < 2 || e > 252) {
+    back = 1.f;
+    return 1.f;
+  }
+  back = __uint_as_float(e << 23);
+  return __uint_as_float((254u - e) << 23);
+}
+
+// ---------------------------------------------------------------------------------------
+// rows kernel: up to 8 * NT query rows of a K/V head
+// ---------------------------------------------------------------------------------------
+// Bound: HBM, 144 bytes a (key, K/V head).  One CTA takes a (member, K/V head, row block) and one
+// chunk of its keys.  A producer warp brings 128-key tiles into a ring of shared-memory stages, one
+// bulk copy per page (K and V of a head lie together in a page); four warps take 32 keys of a tile
+// each.  Both products run transposed on mma.m16n8k16 -- S^T = K Q^T and O^T = V^T P^T -- so that the
+// keys and the head dimension fill the 16-row side and eight query rows the 8-column side: a single
+// query row wastes 7/8 of an otherwise idle tensor pipe and no memory traffic, and a fragment of K or
+// V is dequantised once whatever the number of rows.
+//
+// Fragments come straight from the packed bytes because the products' inner index may be permuted:
+//  * S^T: lane (g, c) (g = lane / 4, c = lane % 4) reads 16 bytes, elements 32c .. 32c+31, of keys g
+//    and g + 8; the m16n8k16 step s takes its bytes 2s and 2s+1.  Q's fragments are loaded by the same
+//    rule.
+//  * O^T: lane (g, c) needs elements 16g .. 16g+15 (one scale block) of four keys; the low nibbles of
+//    two keys' bytes merged by a bit select are an fp16 pair along the keys after one conversion.
+//  * the probabilities pass from S^T's accumulators to P^T's operand by movmatrix (8 x 8 transposes).
+// Which key of an 8-row group sits at index i (key_of) is chosen so that both the 16-byte reads of K
+// and the 8-byte reads of V spread over the shared-memory banks.
+constexpr int kRowWarps = 4;
+constexpr int kRowThreads = 32 * (kRowWarps + 1);
+constexpr int kStages = 3;
+
+__device__ __forceinline__ int key_of(int i) { return (0x65742130u >> (4 * i)) & 7; }  // 0 3 1 2 4 7 5 6
+
+__device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t h2_pack(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+      "r"(bytes), "r"(bar)
+      : "memory");
+}
+
+struct RowsShared {
+  alignas(128) unsigned char stage[kStages][kTileBytes];
+  alignas(8) unsigned long long full[kStages], empty[kStages];
+  uint32_t bad[kStages];  // bit s: segment (page) s of the tile is not in the pool
+  int abort;
+};
+
+template <int NT>
+__global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_constant__ AParams p) {
+  constexpr int R = 8 * NT;
+  extern __shared__ unsigned char smem_raw[];
+  RowsShared& sh = *reinterpret_cast<RowsShared*>(
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127)));
+  volatile int* abort_flag = &sh.abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      bar_init(saddr(&sh.full[s]), 1);
+      bar_init(saddr(&sh.empty[s]), kRowWarps);
+    }
+    sh.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+
+  // CTA -> (unit, chunk): the row blocks of a (member, head, chunk) are neighbours, so that the keys
+  // they share come from L2.
+  int64_t at = blockIdx.x;
+  const int rb = static_cast<int>(at % p.row_blocks);
+  at /= p.row_blocks;
+  const int chunk = static_cast<int>(at % p.chunks);
+  at /= p.chunks;
+  const int b = static_cast<int>(at / p.cache.kv_heads), h = static_cast<int>(at % p.cache.kv_heads);
+  const int64_t unit = at * p.row_blocks + rb;
+
+  pdl_wait();
+  const int n = member_len(p, b);
+  const int row0 = rb * R, row_end = min(row0 + R, p.rows);
+  const int lim_low = token_limit(p, n, row0 / p.group);               // fewest keys of any row of the block
+  const int lim_top = token_limit(p, n, (row_end - 1) / p.group);      // most keys
+  const int tiles = (lim_top + kTileKeys - 1) / kTileKeys;
+  const int j0 = static_cast<int>(static_cast<int64_t>(chunk) * tiles / p.chunks);
+  const int j1 = static_cast<int>(static_cast<int64_t>(chunk + 1) * tiles / p.chunks);
+  const int shift = p.cache.shift, page_rows = 1 << shift;
+  const int segs = kTileKeys >> shift;  // pages per tile
+  const uint32_t seg_bytes = static_cast<uint32_t>(p.cache.head_bytes);
+
+  if (warp == kRowWarps) {
+    // ------------------------------- producer -------------------------------
+    int t = 0;
+    for (int j = j0; j < j1; ++j, ++t) {
+      const int s = t % kStages;
+      // The page first: its latency overlaps the wait for the stage.
+      int64_t page = -1;
+      const int64_t first = (static_cast<int64_t>(j) << 7 >> shift) + lane;
+      const bool mine = lane < segs && (first << shift) < lim_top;
+      if (mine) page = kv4_page(p.cache, b * p.cache.table_pages + first);
+      const unsigned valid = __ballot_sync(0xffffffffu, page >= 0);
+      const unsigned wanted = __ballot_sync(0xffffffffu, mine);
+      if (t >= kStages &&
+          !warp_wait(saddr(&sh.empty[s]), ((t / kStages) & 1) ^ 1, abort_flag, lane))
+        break;
+      const uint32_t bar = saddr(&sh.full[s]);
+      if (lane == 0) {
+        sh.bad[s] = wanted & ~valid;
+        bar_expect_tx(bar, __popc(valid) * seg_bytes);
+      }
+      __syncwarp();
+      if (page >= 0) bulk_load(saddr(sh.stage[s]) + lane * seg_bytes, kv4_head(p.cache, page, h), seg_bytes, bar);
+    }
+    pdl_trigger();
+    // Every copy has landed before the CTA may exit (the consumers have waited for theirs unless the
+    // CTA aborted).
+    volatile int never = 0;
+    for (int u = t > kStages ? t - kStages : 0; u < t; ++u)
+      wait_bar(saddr(&sh.full[u % kStages]), (u / kStages) & 1, &never, lane == 0);
+    __syncwarp();
+  }
+
+  // ------------------------------- consumers -------------------------------
+  const int g = lane >> 2, c = lane & 3;
+  float o[NT][8][4];
+  float m[NT][2], l[NT][2];
+#pragma unroll
+  for (int x = 0; x < NT; ++x) {
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[x][t][e] = 0.f;
+    m[x][0] = m[x][1] = -INFINITY;
+    l[x][0] = l[x][1] = 0.f;
+  }
+  if (warp < kRowWarps) {
+    // Q: query row g of each group of eight, elements 32c .. 32c+31, scaled to fp16.
+    uint32_t qf[NT][16];
+    float qs[NT][2];   // score scale of the query rows 2c, 2c + 1
+    int lim[NT][2];
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      const int r = row0 + 8 * x + g;
+      uint4 w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = make_uint4(0, 0, 0, 0);
+      if (r < row_end) {
+        const int t = r / p.group;
+        const __nv_bfloat16* src =
+            p.q + b * p.q_member + t * p.q_row + (h * p.group + (r - t * p.group)) * kKv4D + 32 * c;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint4*>(src + 8 * i);
+      }
+      const uint32_t* v = reinterpret_cast<const uint32_t*>(w);
+      uint32_t top = v[0] & 0x7fff7fffu;
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top = __vmaxu2(top, v[i] & 0x7fff7fffu);
+      top = max(top << 16, top & 0xffff0000u);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      float back;
+      const float power = row_power(__uint_as_float(top), back);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        qf[x][i] = h2_pack(__uint_as_float(v[i] << 16) * power, __uint_as_float(v[i] & 0xffff0000u) * power);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        qs[x][e] = __shfl_sync(0xffffffffu, back, (2 * c + e) * 4) * p.scale_log2;
+        const int rq = row0 + 8 * x + 2 * c + e;
+        lim[x][e] = rq < row_end ? token_limit(p, n, rq / p.group) : n;
+      }
+    }
+    const int kg = key_of(g);                                   // K rows of this lane: kg, kg + 8
+    const int v0 = key_of(2 * c), v1 = key_of(2 * c + 1);       // V rows: v0, v1, v0 + 8, v1 + 8
+    const int k_codes = kg * 64 + c * 16, k_scale = page_rows * 64 + kg * 8 + c * 2;
+    const int v_base = page_rows * kKv4Row;
+    const int v_codes = v_base + g * 8, v_scale = v_base + page_rows * 64 + g;
+
+    int t = 0;
+    for (int j = j0; j < j1; ++j, ++t) {
+      const int s = t % kStages;
+      if (!warp_wait(saddr(&sh.full[s]), (t / kStages) & 1, abort_flag, lane)) break;
+      const uint32_t bad = *reinterpret_cast<volatile uint32_t*>(&sh.bad[s]);
+      const bool masked = (j + 1) * kTileKeys > lim_low || bad != 0;
+      float acc[2][NT][4];
+      // S^T of this warp's 32 keys, two steps of 16.
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int key = warp * 32 + u * 16;
+        const unsigned char* base = sh.stage[s] + (key >> shift) * seg_bytes;
+        const int in0 = key & (page_rows - 1);
+        const unsigned char* kc = base + in0 * 64 + k_codes;
+        const unsigned char* ksc = base + in0 * 8 + k_scale;
+        const uint4 w0 = *reinterpret_cast<const uint4*>(kc);
+        const uint4 w1 = *reinterpret_cast<const uint4*>(kc + 8 * 64);
+        const uint32_t s0 = kv4_scales(*reinterpret_cast<const uint16_t*>(ksc));
+        const uint32_t s1 = kv4_scales(*reinterpret_cast<const uint16_t*>(ksc + 8 * 8));
+        const uint32_t s0l = __byte_perm(s0, s0, 0x1010), s0h = __byte_perm(s0, s0, 0x3232);
+        const uint32_t s1l = __byte_perm(s1, s1, 0x1010), s1h = __byte_perm(s1, s1, 0x3232);
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[u][x][e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t x0[4], x1[4];
+          kv4_unpack(i == 0 ? w0.x : i == 1 ? w0.y : i == 2 ? w0.z : w0.w, x0);
+          kv4_unpack(i == 0 ? w1.x : i == 1 ? w1.y : i == 2 ? w1.z : w1.w, x1);
+          const uint32_t sa = i < 2 ? s0l : s0h, sb = i < 2 ? s1l : s1h;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t a[4] = {h2_mul(x0[2 * k], sa), h2_mul(x1[2 * k], sb), h2_mul(x0[2 * k + 1], sa),
+                                   h2_mul(x1[2 * k + 1], sb)};
+#pragma unroll
+            for (int x = 0; x < NT; ++x) mma16816(acc[u][x], a, qf[x][4 * i + 2 * k], qf[x][4 * i + 2 * k + 1]);
+          }
+        }
+      }
+      // Scores in log2 units; what a row does not see becomes -inf.
+      bool grow = false;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            acc[u][x][e] *= qs[x][e & 1];
+            if (masked) {
+              const int in_tile = warp * 32 + u * 16 + kg + (e >> 1) * 8;
+              if (j * kTileKeys + in_tile >= lim[x][e & 1] || ((bad >> (in_tile >> shift)) & 1)) acc[u][x][e] = -INFINITY;
+            }
+            grow |= acc[u][x][e] > m[x][e & 1] + 8.f;
+          }
+      // The reference of a row moves only when a score exceeds it by more than 8 (probabilities are
+      // exact for any reference; fp16 holds them up to 2^8 with the same relative rounding).
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = fmaxf(fmaxf(acc[0][x][e], acc[0][x][e + 2]), fmaxf(acc[1][x][e], acc[1][x][e + 2]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            const float next = fmaxf(m[x][e], top);
+            const float alpha = next == -INFINITY ? 1.f : fast_exp2(m[x][e] - next);
+            m[x][e] = next;
+            l[x][e] *= alpha;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              o[x][q][e] *= alpha;
+              o[x][q][e + 2] *= alpha;
+            }
+          }
+      }
+      uint32_t pb[2][NT][2];
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
+        const float r0 = m[x][0] == -INFINITY ? 0.f : m[x][0], r1 = m[x][1] == -INFINITY ? 0.f : m[x][1];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float p0 = fast_exp2(acc[u][x][0] - r0), p1 = fast_exp2(acc[u][x][1] - r1);
+          const float p2 = fast_exp2(acc[u][x][2] - r0), p3 = fast_exp2(acc[u][x][3] - r1);
+          l[x][0] += p0 + p2;
+          l[x][1] += p1 + p3;
+          pb[u][x][0] = transpose8(h2_pack(p0, p1));
+          pb[u][x][1] = transpose8(h2_pack(p2, p3));
+        }
+      }
+      // O^T += V^T P^T.
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int key = warp * 32 + u * 16;
+        const unsigned char* base = sh.stage[s] + (key >> shift) * seg_bytes;
+        const int in0 = key & (page_rows - 1);
+        uint2 w[4];
+        uint32_t sc[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = in0 + (i & 1 ? v1 : v0) + (i >> 1) * 8;
+          w[i] = *reinterpret_cast<const uint2*>(base + v_codes + r * 64);
+          sc[i] = base[v_scale + r * 8];
+        }
+        if (masked) {  // rows that no query row sees and rows of a missing page hold anything: 0 * code = 0
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int in_tile = key + (i & 1 ? v1 : v0) + (i >> 1) * 8;
+            if (j * kTileKeys + in_tile >= lim_top || ((bad >> (in_tile >> shift)) & 1)) sc[i] = 0;
+          }
+        }
+        const uint32_t sa = kv4_scales(sc[0] | (sc[1] << 8)), sb = kv4_scales(sc[2] | (sc[3] << 8));
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t a0 = half ? w[0].y : w[0].x, a1 = half ? w[1].y : w[1].x;
+          const uint32_t b0 = half ? w[2].y : w[2].x, b1 = half ? w[3].y : w[3].x;
+          constexpr uint32_t kLow = 0x0f0f0f0fu;
+          uint32_t al[4], ah[4], bl[4], bh[4];
+          kv4_unpack((a0 & kLow) | ((a1 << 4) & ~kLow), al);
+          kv4_unpack(((a0 >> 4) & kLow) | (a1 & ~kLow), ah);
+          kv4_unpack((b0 & kLow) | ((b1 << 4) & ~kLow), bl);
+          kv4_unpack(((b0 >> 4) & kLow) | (b1 & ~kLow), bh);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t a[4] = {h2_mul(al[i], sa), h2_mul(ah[i], sa), h2_mul(bl[i], sb), h2_mul(bh[i], sb)};
+#pragma unroll
+            for (int x = 0; x < NT; ++x) mma16816(o[x][half * 4 + i], a, pb[u][x][0], pb[u][x][1]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) bar_arrive(saddr(&sh.empty[s]));
+    }
+    // The rows' sums over the lanes that share them.
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[x][e] += __shfl_xor_sync(0xffffffffu, l[x][e], d);
+  }
+  // The four warps' results meet in the stages' memory: no copy is in flight any more.
+  __syncthreads();
+  constexpr int kStride = kKv4D + 4;
+  float* part = reinterpret_cast<float*>(sh.stage);                        // [warp][R][kStride]
+  float2* stat = reinterpret_cast<float2*>(part + kRowWarps * R * kStride);  // [warp][R]
+  static_assert((kRowWarps * R * kStride + 2 * kRowWarps * R) * 4 <= kStages * kTileBytes, "merge buffer");
+  if (warp < kRowWarps) {
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * x + 2 * c + e;
+        float* dst = part + (warp * R + r) * kStride + 16 * g;
+#pragma unroll
+        for (int q = 0; q < 8; q += 2)
+          *reinterpret_cast<float4*>(dst + 2 * q) =
+              make_float4(o[x][q][e], o[x][q][e + 2], o[x][q + 1][e], o[x][q + 1][e + 2]);
+        if (g == 0) stat[warp * R + r] = make_float2(m[x][e], l[x][e]);
+      }
+  }
+  __syncthreads();
+  if (warp == kRowWarps) return;
+  for (int r = warp; r < row_end - row0; r += kRowWarps) {
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, stat[w * R + r].x);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) {
+      const float2 ml = stat[w * R + r];
+      // A warp that saw nothing has a zero sum; a NaN score leaves its reference at -inf and a NaN sum.
+      const float f = ml.x == top || ml.y == 0.f ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - top);
+      const float4 y = *reinterpret_cast<const float4*>(part + (w * R + r) * kStride + 4 * lane);
+      if (ml.y == 0.f) continue;
+      sum += f * ml.y;
+      x.x += f * y.x;
+      x.y += f * y.y;
+      x.z += f * y.z;
+      x.w += f * y.w;
+    }
+    if (p.chunks > 1) {
+      const int64_t slot = (unit * p.chunks + chunk) * R + r;
+      *reinterpret_cast<float4*>(p.ws_o + slot * kKv4D + 4 * lane) = x;
+      if (lane == 0) p.ws_ml[slot] = make_float2(top, sum);
+    } else {
+      const float inv = sum == 0.f ? 0.f : p.cache.v_scale / sum;
+      const int row = row0 + r, t = row / p.group;
+      __nv_bfloat16* dst =
+          p.out + b * p.out_member + t * p.out_row + (h * p.group + (row - t * p.group)) * kKv4D + 4 * lane;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(Pairs16<__nv_bfloat16>::pack_pair(x.x * inv, x.y * inv),
+                                                  Pairs16<__nv_bfloat16>::pack_pair(x.z * inv, x.w * inv));
+    }
+  }
+}
+
+// Merges the key chunks of a query row: out = v_scale * sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c.
+// A warp per row; `block_rows` rows per unit in the workspace.
+__global__ void __launch_bounds__(128) kv4_combine_kernel(const __grid_constant__ AParams p, int block_rows) {
+  const int lane = threadIdx.x & 31;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int64_t bh = at / p.rows;  // (member, K/V head)
+  if (bh >= p.units / p.row_blocks) return;
+  const int row = static_cast<int>(at - bh * p.rows);
+  const int rb = row / block_rows;
+  const int64_t slot0 = (bh * p.row_blocks + rb) * p.chunks * block_rows + (row - rb * block_rows);
+  pdl_wait();
+  float top = -INFINITY;
+  float2 ml[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int ch = lane + 32 * i;
+    ml[i] = ch < p.chunks ? p.ws_ml[slot0 + static_cast<int64_t>(ch) * block_rows] : make_float2(-INFINITY, 0.f);
+    top = fmaxf(top, ml[i].x);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  float f[2], sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    f[i] = ml[i].y == 0.f ? 0.f : (ml[i].x == top ? 1.f : fast_exp2(ml[i].x - top));
+    sum += f[i] * ml[i].y;
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float* src = p.ws_o + slot0 * kKv4D + 4 * lane;
+#pragma unroll 4
+  for (int ch = 0; ch < p.chunks; ++ch) {
+    const float w = __shfl_sync(0xffffffffu, ch < 32 ? f[0] : f[1], ch & 31);
+    if (w == 0.f) continue;  // a chunk in which the row saw nothing (its sums may not have been written)
+    const float4 y = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(ch) * block_rows * kKv4D);
+    x.x += w * y.x;
+    x.y += w * y.y;
+    x.z += w * y.z;
+    x.w += w * y.w;
+  }
+  const float inv = sum == 0.f ? 0.f : p.cache.v_scale / sum;
+  const int b = static_cast<int>(bh / p.cache.kv_heads), h = static_cast<int>(bh % p.cache.kv_heads);
+  const int t = row / p.group;
+  __nv_bfloat16* dst = p.out + b * p.out_member + t * p.out_row + (h * p.group + (row - t * p.group)) * kKv4D + 4 * lane;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(Pairs16<__nv_bfloat16>::pack_pair(x.x * inv, x.y * inv),
+                                              Pairs16<__nv_bfloat16>::pack_pair(x.z * inv, x.w * inv));
+}
+
+// ---------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------
+struct APlan {
+  AParams params;
+  int kernel;       // ps_kv4_kernel, resolved
+  int block_rows;   // query rows of a block (workspace)
+  int64_t ws_bytes;
+};
+
+static int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess &&
+      n > 0)
+    return n;
+  return 148;
+}
+
+// Key chunks per unit: the least modelled time, in tile times of one CTA.  `slots` CTAs run at once; a
+// CTA takes about three tile times to start and finish; partial results cost a second launch.
+static int choose_chunks(int64_t units, int tiles, int64_t slots) {
+  int best = 1;
+  double best_cost = 0;
+  for (int c = 1; c <= kMaxChunks && c <= tiles; ++c) {
+    const int64_t waves = (units * c + slots - 1) / slots;
+    const double cost = static_cast<double>(waves) * ((tiles + c - 1) / c + 3) + (c > 1 ? 4 : 0);
+    if (c == 1 || cost < best_cost) {
+      best = c;
+      best_cost = cost;
+    }
+  }
+  return best;
+}
+
+static int check_rows(const void* ptr, int64_t member, int64_t row, int64_t C, int64_t members, int64_t rows,
+                      const char* name) {
+  if (!ptr) return fail(PS_ERR_NULL, "%s is NULL", name);
+  if (!aligned16(ptr)) return fail(PS_ERR_ALIGN, "%s is not 16-byte aligned", name);
+  if (row < C) return fail(PS_ERR_SHAPE, "%s row stride %lld is below its %lld columns", name, (long long)row, (long long)C);
+  if ((row * 2) % 16 || (members > 1 && (member * 2) % 16))
+    return fail(PS_ERR_ALIGN, "%s strides must be multiples of 16 bytes", name);
+  if (members > 1 && member < rows * row)
+    return fail(PS_ERR_SHAPE, "%s member stride %lld overlaps %lld rows", name, (long long)member, (long long)rows);
+  return PS_OK;
+}
+
+static int build_attn(const ps_kv4_attn_args* a, APlan* plan, bool host_only) {
+  clear_error();
+  if (!a) return fail(PS_ERR_NULL, "args is NULL");
+  memset(plan, 0, sizeof(*plan));
+  AParams& p = plan->params;
+  int64_t cache_rows = 0;
+  int rc = kv4_check_cache(a->cache, &p.cache, &cache_rows);
+  if (rc) return rc;
+  const int hk = a->cache.kv_heads;
+  if (a->heads < 1 || a->heads % hk)
+    return fail(PS_ERR_SHAPE, "heads=%d is not a multiple of kv_heads=%d", a->heads, hk);
+  if (a->q_tokens < 0 || a->kv_tokens < 0 || a->causal_block < 0)
+    return fail(PS_ERR_SHAPE, "q_tokens=%d kv_tokens=%d causal_block=%d", a->q_tokens, a->kv_tokens, a->causal_block);
+  if (a->kv_tokens > a->cache.table_pages * a->cache.page_rows)
+    return fail(PS_ERR_BOUNDS, "kv_tokens=%d exceeds a member's %lld cache rows", a->kv_tokens,
+                (long long)(a->cache.table_pages * a->cache.page_rows));
+  if (a->kernel != PS_KV4_AUTO && a->kernel != PS_KV4_ROWS && a->kernel != PS_KV4_TILES)
+    return fail(PS_ERR_SHAPE, "kernel %d unknown", a->kernel);
+  if (a->key_chunks < 0 || a->key_chunks > kMaxChunks)
+    return fail(PS_ERR_SHAPE, "key_chunks=%d (0..%d)", a->key_chunks, kMaxChunks);
+  const int64_t C = static_cast<int64_t>(a->heads) * kKv4D;
+  if ((rc = check_rows(a->q, a->q_member_stride, a->q_row_stride, C, a->cache.members, a->q_tokens, "q")) ||
+      (rc = check_rows(a->out, a->out_member_stride, a->out_row_stride, C, a->cache.members, a->q_tokens, "out")))
+    return rc;
+  if (reinterpret_cast<uintptr_t>(a->kv_lens) & 3u) return fail(PS_ERR_ALIGN, "kv_lens is not 4-byte aligned");
+  p.q = static_cast<const __nv_bfloat16*>(a->q);
+  p.out = static_cast<__nv_bfloat16*>(a->out);
+  p.lens = a->kv_lens;
+  p.q_member = a->q_member_stride; p.q_row = a->q_row_stride;
+  p.out_member = a->out_member_stride; p.out_row = a->out_row_stride;
+  p.Lq = a->q_tokens;
+  p.kv_max = a->kv_tokens;
+  p.causal_block = a->causal_block;
+  p.group = a->heads / hk;
+  const int64_t rows = static_cast<int64_t>(a->q_tokens) * p.group;
+  if (rows > (1 << 30)) return fail(PS_ERR_UNSUPPORTED, "%lld query rows of a K/V head", (long long)rows);
+  p.rows = static_cast<int32_t>(rows);
+  plan->kernel = PS_KV4_ROWS;
+  plan->block_rows = rows <= 8 ? 8 : 16;
+  p.row_blocks = (p.rows + plan->block_rows - 1) / plan->block_rows;
+  p.units = a->cache.members * hk * p.row_blocks;
+  const int tiles = (a->kv_tokens + kTileKeys - 1) / kTileKeys;
+  const int sms = host_only ? 148 : sm_count();
+  int chunks = a->key_chunks > 0 ? a->key_chunks : choose_chunks(p.units, tiles, 3ll * sms);
+  if (chunks > tiles) chunks = tiles > 0 ? tiles : 1;
+  p.chunks = chunks;
+  const double scale = a->scale > 0.f ? a->scale : 1.0 / sqrt(static_cast<double>(kKv4D));
+  p.scale_log2 = static_cast<float>(scale * a->cache.k_scale * 1.4426950408889634);
+  if (p.units > (1 << 28) || p.units * p.chunks > 0x7fffffffLL)
+    return fail(PS_ERR_UNSUPPORTED, "grid of %lld CTAs", (long long)(p.units * p.chunks));
+  const int64_t slots = p.units * p.chunks * plan->block_rows;
+  plan->ws_bytes = p.chunks > 1 ? slots * (kKv4D * 4 + 8) : 0;
+  if (!host_only && plan->ws_bytes > 0) {
+    if (!a->workspace || a->workspace_bytes < plan->ws_bytes)
+      return fail(PS_ERR_NULL, "workspace of %lld bytes needed (ps_kv4_attention_workspace), %lld given",
+                  (long long)plan->ws_bytes, (long long)a->workspace_bytes);
+    if (!aligned16(a->workspace)) return fail(PS_ERR_ALIGN, "workspace is not 16-byte aligned");
+  }
+  p.ws_o = static_cast<float*>(a->workspace);
+  p.ws_ml = reinterpret_cast<float2*>(static_cast<unsigned char*>(a->workspace) + slots * kKv4D * 4);
+  return PS_OK;
+}
+
+// Opts `fn` into `bytes` of dynamic shared memory, once per device.
+static cudaError_t allow_smem(const void* fn, int bytes) {
+  static const void* done[64][4];
+  static std::mutex lock;
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  std::lock_guard<std::mutex> guard(lock);
+  if (dev >= 0 && dev < 64)
+    for (const void*& f : done[dev]) {
+      if (f == fn) return cudaSuccess;
+      if (!f) {
+        err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (err == cudaSuccess) f = fn;
+        return err;
+      }
+    }
+  return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+template <typename... A>
+static cudaError_t launch(void (*fn)(A...), int64_t blocks, int threads, int smem, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, fn, args...);
+}
+
+}  // namespace
+
+cudaError_t kv4_attention_counts(uint32_t* counts, bool reset) { return kv4_take_counts(counts, reset); }
+
+}  // namespace ps
+
+extern "C" int32_t ps_kv4_attention_validate(const ps_kv4_attn_args* args) {
+  ps::APlan plan;
+  return ps::build_attn(args, &plan, true);
+}
+
+extern "C" int32_t ps_kv4_attention_workspace(const ps_kv4_attn_args* args, int64_t* bytes) {
+  if (!bytes) return ps::fail(PS_ERR_NULL, "bytes is NULL");
+  ps::APlan plan;
+  const int rc = ps::build_attn(args, &plan, true);
+  if (rc == PS_OK) *bytes = plan.ws_bytes;
+  return rc;
+}
+
+extern "C" int32_t ps_attention_kv4(const ps_kv4_attn_args* args, void* stream) {
+  ps::APlan plan;
+  const int rc = ps::build_attn(args, &plan, false);
+  if (rc != PS_OK || plan.params.units == 0) return rc;
+  const ps::AParams& p = plan.params;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int smem = static_cast<int>(sizeof(ps::RowsShared)) + 128;
+  auto fn = plan.block_rows == 8 ? ps::kv4_rows_kernel<1> : ps::kv4_rows_kernel<2>;
+  cudaError_t err = ps::allow_smem(reinterpret_cast<const void*>(fn), smem);
+  if (err == cudaSuccess) err = ps::launch(fn, p.units * p.chunks, ps::kRowThreads, smem, s, p);
+  if (err == cudaSuccess && p.chunks > 1) {
+    const int64_t rows = p.units / p.row_blocks * p.rows;
+    err = ps::launch(ps::kv4_combine_kernel, (rows + 3) / 4, 128, 0, s, p, plan.block_rows);
+  }
+  if (err != cudaSuccess) return ps::fail(PS_ERR_LAUNCH, "kv4 attention launch: %s", cudaGetErrorString(err));
+  return PS_OK;
+}

@@ -1,4 +1,4 @@
-"""Torch-facing wrappers of the native sm_100a kernels (``include/physis_b200.h``).
+"""Torch-facing wrappers of the native sm_100a kernels (the headers under ``include/``).
 
 Tensors are passed to the C ABI as raw device pointers plus element strides; every
 launch goes on the current CUDA stream of the tensors' device.  These wrappers
@@ -13,7 +13,7 @@ import ctypes
 import inspect
 import struct
 from dataclasses import dataclass
-from typing import Sequence
+from typing import NamedTuple, Sequence
 
 import torch
 
@@ -680,6 +680,358 @@ def attention_timeouts(reset: bool = True, device: int | None = None) -> int:
     with _on_device(index):
         _check(_lib.load().ps_attention_timeouts(ctypes.byref(count), int(reset)))
     return int(count.value)
+
+
+# --------------------------------------------------------------------------------------
+# Paged 4-bit K/V cache (include/physis_b200_kv4.h)
+# --------------------------------------------------------------------------------------
+KV4_HEAD_DIM = 128
+KV4_ROW_BYTES = _lib.KV4_ROW_BYTES
+KV4_PAGE_ROWS = (16, 32, 64, 128)
+_KV4_KERNELS = {"auto": _lib.KV4_AUTO, "rows": _lib.KV4_ROWS, "tiles": _lib.KV4_TILES}
+_KV4_CACHE = "QQqqqiiff"
+_PREP4_HEAD = "=8if3iq"
+_PREP4 = struct.Struct(_PREP4_HEAD + "Qq" * 3 + "QQQQq" + "Qq" * 2 + "Qqq" + _KV4_CACHE + "Q")
+_READ4 = struct.Struct("=iiqq" + "Qqq" * 2 + _KV4_CACHE)
+_ATTN4_HEAD = "=4if3i" + "Qqq" * 2 + "Q"
+_ATTN4 = struct.Struct(_ATTN4_HEAD + "Qq" + _KV4_CACHE)
+_ATTN4_WORKSPACE = struct.calcsize(_ATTN4_HEAD)
+
+
+def kv4_pages(num_pages: int, kv_heads: int, page_rows: int = 128, device=None) -> torch.Tensor:
+    """A pool of ``num_pages`` zeroed pages, uint8 [num_pages, kv_heads, 2, page_rows * 72]: for each
+    head K and V, ``page_rows`` rows of 64 code bytes (e2m1, two elements a byte), then of 8 scale
+    bytes (e4m3, one per 16 elements)."""
+    if page_rows not in KV4_PAGE_ROWS:
+        raise PrepError(f"page_rows={page_rows} is not one of {KV4_PAGE_ROWS}")
+    return torch.zeros(num_pages, kv_heads, 2, page_rows * KV4_ROW_BYTES, dtype=torch.uint8, device=device)
+
+
+def _kv4_cache(pages: torch.Tensor, table: torch.Tensor, k_scale: float, v_scale: float):
+    """(device index, members, page_rows, ``ps_kv4_cache`` fields) of a pool and a page table."""
+    if pages.dtype is not torch.uint8 or pages.dim() != 4 or pages.shape[2] != 2 or not pages.is_contiguous():
+        raise PrepError("pages must be a contiguous uint8 [pages, kv_heads, 2, page_rows * 72] tensor, got "
+                        f"{pages.dtype} {tuple(pages.shape)}")
+    page_rows, rest = divmod(pages.shape[3], KV4_ROW_BYTES)
+    if rest or page_rows not in KV4_PAGE_ROWS:
+        raise PrepError(f"pages of {pages.shape[3]} bytes a head: page_rows * {KV4_ROW_BYTES} with page_rows one of "
+                        f"{KV4_PAGE_ROWS}")
+    if table.dtype is not torch.int32 or table.dim() != 2 or not table.is_contiguous():
+        raise PrepError(f"table must be a contiguous int32 [members, pages] tensor, got {table.dtype} "
+                        f"{tuple(table.shape)}")
+    if not pages.is_cuda or not table.is_cuda:
+        raise PrepError("the 4-bit cache lives in CUDA tensors only (there is no CPU path)")
+    device_index = pages.get_device()
+    if table.get_device() != device_index:
+        raise PrepError(f"tensors on different devices: {pages.device} and {table.device}")
+    members, table_pages = table.shape
+    return device_index, members, page_rows, (pages.data_ptr(), table.data_ptr(), pages.shape[0], members, table_pages,
+                                              pages.shape[1], page_rows, k_scale, v_scale)
+
+
+def _prepare4(
+    *,
+    heads: int,
+    seqs: Sequence[Seq],
+    pages: torch.Tensor,
+    table: torch.Tensor,
+    cos: torch.Tensor | None = None,
+    sin: torch.Tensor | None = None,
+    kv_heads: int | None = None,
+    head_dim: int = KV4_HEAD_DIM,
+    q: torch.Tensor | None = None,
+    k: torch.Tensor | None = None,
+    v: torch.Tensor | None = None,
+    q_weight: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    q_out: torch.Tensor | None = None,
+    k_pre: torch.Tensor | None = None,
+    k_sink: torch.Tensor | None = None,
+    k_scale: float = 1.0,
+    v_scale: float = 1.0,
+    table_mode: str = "axes",
+    axis_split: Sequence[int] | None = None,
+    launch: str = "pdl",
+) -> tuple:
+    """Validate a ``qk_norm_rope_kv4`` call and pack its ``ps_kv4_prep_args`` (one buffer per
+    ``PS_MAX_SEQS`` sequences); returns (device index, [(args, seq buffer)], tensor signatures)."""
+    device_index, _, _, cache = _kv4_cache(pages, table, k_scale, v_scale)
+    hk = pages.shape[1]
+    if kv_heads is not None and kv_heads != hk:
+        raise PrepError(f"kv_heads={kv_heads}, but the pages hold {hk} heads")
+    C, Ck = heads * head_dim, hk * head_dim
+    ref = next((t for t in (q, k, v, k_sink) if t is not None), None)
+    if ref is None:
+        raise PrepError("q, k and v are all None")
+    dtype = _DEVICE_DTYPES.get(ref.dtype)
+    if dtype is None:
+        raise PrepError(f"unsupported dtype {ref.dtype}: the kernels take bfloat16 or float32")
+    for name, t in (("q", q), ("k", k), ("v", v), ("q_out", q_out), ("k_pre", k_pre), ("k_sink", k_sink)):
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise PrepError("the prep kernels run on CUDA tensors only (there is no CPU path)")
+        if t.dtype is not ref.dtype or t.get_device() != device_index:
+            raise PrepError(f"{name} is {t.dtype} on {t.device}, expected {ref.dtype} on {pages.device}")
+    weight_f32, first = 0, None
+    for name, w, width in (("q_weight", q_weight, C), ("k_weight", k_weight, Ck)):
+        if w is None:
+            continue
+        if not w.is_cuda or w.get_device() != device_index:
+            raise PrepError(f"{name} must be a CUDA tensor on {pages.device}")
+        if w.dtype is not ref.dtype and w.dtype is not torch.float32:
+            raise PrepError(f"{name} is {w.dtype}: RMSNorm weights are {ref.dtype} or float32")
+        if first is not None and w.dtype is not first:
+            raise PrepError("q_weight and k_weight differ in dtype")
+        if w.numel() != width or not w.is_contiguous():
+            raise PrepError(f"{name} must be a contiguous [{width}] vector")
+        first, weight_f32 = w.dtype, int(w.dtype is torch.float32)
+    launch_code = _LAUNCH.get(launch)
+    if launch_code is None:
+        raise PrepError(f"launch {launch!r} is not one of {sorted(_LAUNCH)}")
+    for name, t in (("cos", cos), ("sin", sin)):
+        if t is None:
+            continue
+        if t.dtype is not torch.float32:
+            raise PrepError(f"{name} must be float32")
+        if t.get_device() != device_index:
+            raise PrepError(f"{name} must be on {pages.device}")
+        if t.shape[-1] != head_dim or not t.is_contiguous():
+            raise PrepError(f"{name} must be contiguous with last dimension head_dim={head_dim}")
+    if (cos is None) != (sin is None) or (cos is not None and cos.shape != sin.shape):
+        raise PrepError("cos and sin differ in shape")
+    if table_mode == "axes":
+        mode = _lib.TABLE_AXES
+        split = tuple(axis_split) if axis_split is not None else _default_split(head_dim)
+    elif table_mode == "tokens":
+        mode, split = _lib.TABLE_TOKENS, (0, 0, 0)
+    else:
+        raise PrepError(f"table_mode {table_mode!r} is not 'axes' or 'tokens'")
+    qp, qs, q_rows = _rows(q, C, "q")
+    kp, ks, k_rows = _rows(k, Ck, "k")
+    vp, vs, v_rows = _rows(v, Ck, "v")
+    qop, qos, qo_rows = _rows(q_out, C, "q_out")
+    kpp, kps, kp_rows = _rows(k_pre, Ck, "k_pre")
+    ksp, kss, ks_rows = _rows(k_sink, Ck, "k_sink")
+    in_rows = min([r for r, t in ((q_rows, q), (k_rows, k), (v_rows, v), (qo_rows, q_out), (kp_rows, k_pre))
+                   if t is not None] or [0])
+    qw = 0 if q_weight is None else q_weight.data_ptr()
+    kw = 0 if k_weight is None else k_weight.data_ptr()
+    cp, sp, table_rows = (0, 0, 0) if cos is None else (cos.data_ptr(), sin.data_ptr(), cos.numel() // head_dim)
+    seqs = list(seqs)
+    parts = []
+    for begin in range(0, max(1, len(seqs)), _lib.MAX_SEQS):
+        part = seqs[begin:begin + _lib.MAX_SEQS]
+        seq_buf = ctypes.create_string_buffer(_SEQ.size * max(1, len(part)))
+        for i, sq in enumerate(part):
+            _SEQ.pack_into(seq_buf, i * _SEQ.size, sq.token_start, sq.n_tokens, sq.grid_h, sq.grid_w,
+                           sq.frame_offset, sq.table_row, sq.ring_row, sq.ring_frames, sq.ring_slot0, sq.kind, 0)
+        args = ctypes.create_string_buffer(_PREP4.size)
+        _PREP4.pack_into(args, 0, dtype, heads, head_dim, mode, split[0], split[1], split[2], len(part), float(eps),
+                         weight_f32, launch_code, 0, in_rows, qp or 0, qs, kp or 0, ks, vp or 0, vs, qw, kw, cp, sp,
+                         table_rows, qop or 0, qos, kpp or 0, kps, ksp or 0, kss, ks_rows, *cache,
+                         ctypes.addressof(seq_buf))
+        parts.append((args, seq_buf))
+    signatures = {name: _signature(t) for name, t in (("q", q), ("k", k), ("v", v), ("q_weight", q_weight),
+                                                      ("k_weight", k_weight), ("q_out", q_out))}
+    return device_index, parts, signatures
+
+
+def qk_norm_rope_kv4(**kwargs) -> None:
+    """``qk_norm_rope_kv`` with a paged 4-bit cache in the place of the ring: RMSNorm of Q and K, RoPE,
+    and the quantised write of rotated K and of V, one launch per ``PS_MAX_SEQS`` sequences
+    (``ps_qk_norm_rope_kv4``).
+
+    Keyword arguments: ``heads`` (query heads), ``seqs`` (``Seq`` list; ``ring_row`` counts cache rows:
+    member b's start at ``b * table.shape[1] * page_rows``), ``pages`` (``kv4_pages``), ``table`` (int32
+    [members, pages per member]: page of each member's rows; entries that no sequence reaches may be
+    anything), ``cos``/``sin``, ``q`` [rows, heads*128], ``k``/``v`` [rows, kv_heads*128] (bfloat16 or
+    float32, any row stride), ``q_weight``/``k_weight``, ``eps``, ``q_out``, ``k_pre``, ``k_sink`` (pre-RoPE
+    K rows of ``SEQ_SINK`` sequences), ``k_scale``/``v_scale`` (tensor scales of the cache: an element is
+    code * block scale * tensor scale, at most 2688 tensor scales), ``table_mode``, ``axis_split`` and
+    ``launch`` as in ``qk_norm_rope_kv``.  NaN is stored as zero and infinities saturate; both, and
+    page numbers outside the pool (their rows are skipped), are counted in ``kv4_counters``.
+    """
+    device_index, parts, _ = _prepare4(**kwargs)
+    lib = _lib.load()
+    with _on_device(device_index):
+        stream = _current_stream(device_index)
+        for args, _seq_buf in parts:
+            _check(lib.ps_qk_norm_rope_kv4(args, stream))
+
+
+qk_norm_rope_kv4.__signature__ = inspect.signature(_prepare4).replace(return_annotation=None)
+
+_PREP4_OFFSETS = {
+    "q": struct.calcsize(_PREP4_HEAD),
+    "k": struct.calcsize(_PREP4_HEAD + "Qq"),
+    "v": struct.calcsize(_PREP4_HEAD + "Qq" * 2),
+    "q_weight": struct.calcsize(_PREP4_HEAD + "Qq" * 3),
+    "k_weight": struct.calcsize(_PREP4_HEAD + "Qq" * 3 + "Q"),
+    "q_out": struct.calcsize(_PREP4_HEAD + "Qq" * 3 + "QQQQq"),
+}
+
+
+class Prep4Plan:
+    """A ``qk_norm_rope_kv4`` call validated and packed once, launched many times (as ``PrepPlan``):
+    ``launch`` swaps q, k, v, the norm weights or q_out for tensors of the planned shape, strides,
+    dtype and device.  Sequences, tables, pages and the page table's address are fixed (the table's
+    entries may change between launches)."""
+
+    def __init__(self, **kwargs):
+        self.device_index, self.parts, self.signatures = _prepare4(**kwargs)
+        # The packed arguments hold raw device pointers: the plan owns every tensor they point at.
+        self._tensors = {name: t for name, t in kwargs.items() if isinstance(t, torch.Tensor)}
+        self._lib = _lib.load()
+
+    def launch(self, **tensors) -> None:
+        """One launch with the given tensors swapped in."""
+        for name, t in tensors.items():
+            want = self.signatures.get(name, False)
+            if want is False:
+                raise PrepError(f"{name} cannot be swapped in a plan (only q, k, v, q_weight, k_weight, q_out)")
+            if want is None or t is None or (t.shape, t.stride(), t.dtype, t.device) != want:
+                raise PrepError(f"{name} must match the planned tensor (shape, strides, dtype, device)")
+        for name, t in tensors.items():
+            for args, _seq_buf in self.parts:
+                struct.pack_into("=Q", args, _PREP4_OFFSETS[name], t.data_ptr())
+            self._tensors[name] = t
+        with _on_device(self.device_index):
+            stream = _current_stream(self.device_index)
+            for args, _seq_buf in self.parts:
+                _check(self._lib.ps_qk_norm_rope_kv4(args, stream))
+
+
+def read_kv4(pages: torch.Tensor, table: torch.Tensor, tokens: int, *, row0: int = 0, k_scale: float = 1.0,
+             v_scale: float = 1.0, dtype: torch.dtype = torch.bfloat16, k_out: torch.Tensor | None = None,
+             v_out: torch.Tensor | None = None):
+    """Rows [row0, row0 + tokens) of every member of a 4-bit cache as numbers (``ps_kv4_read``): K and V,
+    each [members, tokens, kv_heads * 128] of ``dtype`` (bfloat16 or float32), for consumers that read an
+    ordinary window.  ``k_out``/``v_out`` receive them if given (their dtype is then used).  Rows of pages
+    outside the pool read as zero and are counted in ``kv4_counters``."""
+    device_index, members, _, cache = _kv4_cache(pages, table, k_scale, v_scale)
+    C = pages.shape[1] * KV4_HEAD_DIM
+    tokens, row0 = int(tokens), int(row0)
+    if tokens < 0:
+        raise PrepError(f"tokens={tokens}")
+    dtype = next((t.dtype for t in (k_out, v_out) if t is not None), dtype)
+    code = _DEVICE_DTYPES.get(dtype)
+    if code is None:
+        raise PrepError(f"unsupported dtype {dtype}: the kernels write bfloat16 or float32")
+    if k_out is None:
+        k_out = torch.empty(members, tokens, C, dtype=dtype, device=pages.device)
+    if v_out is None:
+        v_out = torch.empty(members, tokens, C, dtype=dtype, device=pages.device)
+    strides = []
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        if t.dtype is not dtype or t.get_device() != device_index:
+            raise PrepError(f"{name} is {t.dtype} on {t.device}, expected {dtype} on {pages.device}")
+        if t.shape[0] != members or t.shape[1] != tokens:
+            raise PrepError(f"{name} must be [{members}, {tokens}, {C}], got {tuple(t.shape)}")
+        strides.append(_member_rows(t, C, name))
+    args = ctypes.create_string_buffer(_READ4.size)
+    # An empty tensor may have no address; the library checks the rest of such a call all the same.
+    _READ4.pack_into(args, 0, code, 0, row0, tokens, k_out.data_ptr() or 16, *strides[0], v_out.data_ptr() or 16,
+                     *strides[1], *cache)
+    with _on_device(device_index):
+        _check(_lib.load().ps_kv4_read(args, _current_stream(device_index)))
+    return k_out, v_out
+
+
+def attention_kv4(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, kv_tokens=None, *, heads: int,
+                  out: torch.Tensor | None = None, scale: float | None = None, k_scale: float = 1.0,
+                  v_scale: float = 1.0, causal_block: int = 0, max_kv_tokens: int | None = None,
+                  kernel: str = "auto", key_chunks: int = 0, workspace: torch.Tensor | None = None,
+                  check_timeouts: bool = False) -> torch.Tensor:
+    """Softmax attention of the query rows over the window rows of a paged 4-bit cache
+    (``ps_attention_kv4``): ``attention`` with the cache in the place of the ring.
+
+    ``q``: [B, Lq, heads*128] (or [B, Lq, heads, 128]) bf16; ``pages`` [pages, kv_heads, 2, page_rows*72]
+    and ``table`` int32 [B, pages per member] as written by ``qk_norm_rope_kv4``; ``heads`` is a multiple
+    of kv_heads, consecutive query heads share a K/V head.  ``kv_tokens``: window rows, one int for all
+    members, an int32 CUDA tensor [B] (read on the device; ``max_kv_tokens``, default the whole table,
+    bounds it and sizes the work split), or None for the whole table.  Zero rows are allowed.
+    ``causal_block`` c > 0 lets query row t see the rows below ``min(n, n - Lq + (t // c + 1) * c)`` of
+    a member's n: 1 is the causal mask, the tokens of a frame let a frame see itself and the frames
+    before it.  A row that sees nothing gets zeros.  Returns ``out`` [B, Lq, heads*128] (allocated if
+    not given).  ``kernel`` ("auto", "rows", "tiles") and ``key_chunks`` override the kernel and the work
+    split; ``workspace`` is a byte tensor for the partial results of key chunks (allocated if None or
+    too small).  ``check_timeouts=True`` synchronises and raises ``PrepError`` if a bounded wait ran out.
+    """
+    device_index, members, page_rows, cache = _kv4_cache(pages, table, k_scale, v_scale)
+    if q.dtype is not torch.bfloat16:
+        raise PrepError("attention takes bfloat16 q")
+    if q.get_device() != device_index:
+        raise PrepError(f"q is on {q.device}, the cache on {pages.device}")
+    C = heads * KV4_HEAD_DIM
+    if q.dim() < 3 or q.shape[0] != members:
+        raise PrepError(f"q must be [{members}, Lq, {C}], got {tuple(q.shape)}")
+    Lq = q.shape[1]
+    code = _KV4_KERNELS.get(kernel)
+    if code is None:
+        raise PrepError(f"kernel {kernel!r} is not one of {sorted(_KV4_KERNELS)}")
+    rows, lens = table.shape[1] * page_rows, 0
+    if kv_tokens is None:
+        kv_tokens = rows
+    elif isinstance(kv_tokens, torch.Tensor):
+        if kv_tokens.dtype is not torch.int32 or kv_tokens.shape != (members,) or not kv_tokens.is_contiguous():
+            raise PrepError(f"kv_tokens must be an int or a contiguous int32 [{members}] tensor")
+        if kv_tokens.get_device() != device_index:
+            raise PrepError(f"kv_tokens is on {kv_tokens.device}, the cache on {pages.device}")
+        lens = kv_tokens.data_ptr()
+        kv_tokens = rows if max_kv_tokens is None else int(max_kv_tokens)
+    else:
+        kv_tokens = int(kv_tokens)
+    if not 0 <= kv_tokens <= rows:
+        raise PrepError(f"kv_tokens={kv_tokens} outside the {rows} rows of the page table")
+    if out is None:
+        out = torch.empty(members, Lq, C, device=q.device, dtype=torch.bfloat16)
+    elif out.dtype is not torch.bfloat16 or out.get_device() != device_index or out.shape[:2] != q.shape[:2]:
+        raise PrepError(f"out must be a bfloat16 [{members}, {Lq}, {C}] tensor on {pages.device}")
+    qs, os_ = _member_rows(q, C, "q"), _member_rows(out, C, "out")
+    if Lq == 0:
+        return out
+    args = ctypes.create_string_buffer(_ATTN4.size)
+    _ATTN4.pack_into(args, 0, heads, Lq, kv_tokens, causal_block, scale or 0.0, code, key_chunks, 0, q.data_ptr(), *qs,
+                     out.data_ptr(), *os_, lens, 0, 0, *cache)
+    lib = _lib.load()
+    with _on_device(device_index):
+        need = ctypes.c_int64(0)
+        _check(lib.ps_kv4_attention_workspace(args, ctypes.byref(need)))
+        if need.value:
+            if workspace is None or workspace.numel() * workspace.element_size() < need.value:
+                workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+            elif workspace.get_device() != device_index or not workspace.is_contiguous():
+                raise PrepError(f"workspace must be a contiguous tensor on {pages.device}")
+            struct.pack_into("=Qq", args, _ATTN4_WORKSPACE, workspace.data_ptr(),
+                             workspace.numel() * workspace.element_size())
+        _check(lib.ps_attention_kv4(args, _current_stream(device_index)))
+    if check_timeouts:
+        count = kv4_counters(reset=True, device=device_index).timeouts
+        if count:
+            raise PrepError(f"{count} bounded wait(s) of the attention kernel ran out on cuda:{device_index}: "
+                            "the outputs of the calls since the last check are undefined")
+    return out
+
+
+class Kv4Counters(NamedTuple):
+    """Counts of ``kv4_counters``."""
+
+    bad_pages: int
+    nonfinite: int
+    timeouts: int
+
+
+def kv4_counters(reset: bool = True, device: int | None = None) -> Kv4Counters:
+    """Counts of the 4-bit cache's kernels on ``device`` since the last reset (synchronises it): accesses to
+    pages outside the pool, blocks of 16 elements that held an infinity or a NaN when they were stored, and
+    bounded waits that ran out (the outputs of the calls since are then undefined)."""
+    index = torch.cuda.current_device() if device is None else int(device)
+    counts = (ctypes.c_uint32 * 3)()
+    with _on_device(index):
+        _check(_lib.load().ps_kv4_counters(counts, int(reset)))
+    return Kv4Counters(*(int(c) for c in counts))
 
 
 def wait_selftest(limit_us: int = 20000, device: int | None = None) -> None:

@@ -1,0 +1,554 @@
+"""GPU tests of the paged 4-bit K/V cache (include/physis_b200_kv4.h) against the 64-bit restatement in
+oracle/kv4.py.
+
+Append: everything that is quantised is reproduced bit for bit (the sum of squares is accumulated in 64
+bits, every later step is an IEEE fp32 operation), so codes and scales have to be equal.  Q is rounded from
+an fp32 sum of another order: within one bf16 ulp, as in the ring's tests.
+
+Read: code * scale has 6 significant bits and is exact; times the tensor scale it is rounded once: within half
+a step of the output type (bf16 2^-8, fp32 2^-24 relative).
+
+Attention, per output element, with p the probabilities and A = sum p |v| (sum p = 1): the output's rounding to
+bf16, 2^-8 |out|; each p's rounding to fp16, 2^-11 relative and so 2^-11 A; each score's fp32 accumulation over
+128 products (128 * 2^-24 * sum |q k| / sqrt(128), below 2^-14 for |q k| sums up to 2^8 * sqrt(128)) and the
+approximate 2^x (2^-22), together below 2^-13 A; a p below fp16's normal range loses at most 2^-25 absolutely
+against a largest p of at least 1, N keys together 2^-25 N max|v|.  Tolerance: 2^-8 |out| + 2^-10 A + 2^-24 N max|v|.
+"""
+import pytest
+import torch
+
+from oracle import kv4, wan_prep
+from physisserve_b200 import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def make_table(members, table_pages, spare, seed):
+    """(number of pages, table): distinct pages in random order, `spare` pages that nobody owns."""
+    n = members * table_pages + spare
+    return n, torch.randperm(n, generator=gen(seed))[:members * table_pages].view(members, table_pages).int()
+
+
+def fill(members, rows, heads, page_rows, seed, k_scale=1.0, v_scale=1.0, extra_pages=1, k_size=1.0):
+    """(pages, table, k fp64, v fp64): a cache filled by the oracle, unowned and unwritten rows full of 0xff
+    (scale bytes that would read as NaN)."""
+    table_pages = -(-rows // page_rows) + extra_pages
+    n, table = make_table(members, table_pages, 2, seed)
+    pages = torch.full((n, heads, 2, page_rows * 72), 0xff, dtype=torch.uint8)
+    g = gen(seed + 1)
+    back = []
+    for which, scale in ((0, k_scale), (1, v_scale)):
+        x = torch.randn(members * rows, heads, 128, generator=g) * (k_size if which == 0 else 1.0)
+        flat = (torch.arange(members)[:, None] * table_pages * page_rows + torch.arange(rows)).flatten()
+        kv4.store(pages, table, flat, x, which, scale)
+        back.append(kv4.load(pages, table, flat, which, scale).view(members, rows, heads, 128))
+    return pages, table, back[0], back[1]
+
+
+# ---------------------------------------------------------------------------------------
+# Append
+# ---------------------------------------------------------------------------------------
+def append_case(streams, gh, gw, frames, heads, hk, page_rows, dtype, ring, seed, k_scale=1.0, v_scale=0.375,
+                fused=False, w32=False, size=1.0, mode="axes"):
+    hw, C, Ck = gh * gw, heads * 128, hk * 128
+    n = hw * frames
+    T = streams * n
+    g = gen(seed)
+    qkv = (torch.randn(T, C + 2 * Ck, generator=g) * size).to(dtype)
+    wdt = torch.float32 if w32 else dtype
+    wq, wk = ((torch.rand(c, generator=g) + 0.5).to(wdt) for c in (C, Ck))
+    cos, sin = wan_prep.rope_tables(128, 256)
+    table_pages = -(-ring * hw // page_rows)
+    pages_n, table = make_table(streams, table_pages, 2, seed)
+    pages = torch.randint(0, 256, (pages_n, hk, 2, page_rows * 72), generator=g, dtype=torch.uint8)
+    offsets = torch.randint(0, 100, (streams,), generator=g).tolist()
+    slots = torch.randint(0, ring, (streams,), generator=g).tolist()
+    seqs, flat, cos_t, sin_t = [], [], [], []
+    for b in range(streams):
+        base = b * table_pages * page_rows
+        seqs.append(ops.Seq(b * n, n, gh, gw, offsets[b], b * n, base, ring, slots[b]))
+        f = torch.arange(n) // hw
+        flat.append(base + ((slots[b] + f) % ring) * hw + torch.arange(n) % hw)
+        c, s = wan_prep.frames_table(cos, sin, wan_prep.axis_dims(128), offsets[b], offsets[b] + frames, gh, gw)
+        cos_t.append(c[0, :, 0])
+        sin_t.append(s[0, :, 0])
+    cos_t, sin_t, flat = torch.cat(cos_t), torch.cat(sin_t), torch.cat(flat)
+
+    dev = qkv.to(DEV)
+    q, k, v = dev.split((C, Ck, Ck), 1)
+    if not fused:
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    tables = (cos, sin) if mode == "axes" else (cos_t.contiguous(), sin_t.contiguous())
+    got_pages, q_out = pages.to(DEV), torch.empty(T, C, dtype=dtype, device=DEV)
+    kwargs = dict(heads=heads, kv_heads=hk, seqs=seqs, cos=tables[0].to(DEV), sin=tables[1].to(DEV), q=q, k=k, v=v,
+                  q_weight=wq.to(DEV), k_weight=wk.to(DEV), eps=1e-6, q_out=q_out, pages=got_pages, table=table.to(DEV),
+                  k_scale=k_scale, v_scale=v_scale, table_mode=mode)
+
+    want = pages.clone()
+    qn, kn = kv4.rms_norm(qkv[:, :C], wq, 1e-6), kv4.rms_norm(qkv[:, C:C + Ck], wk, 1e-6)
+    q_ref = wan_prep.rope(qn.view(1, T, heads, 128), cos_t[None, :, None], sin_t[None, :, None])[0].flatten(1)
+    k_rot = wan_prep.rope(kn.view(1, T, hk, 128), cos_t[None, :, None], sin_t[None, :, None])[0]
+    kv4.store(want, table, flat, k_rot, 0, k_scale)
+    kv4.store(want, table, flat, qkv[:, C + Ck:].view(T, hk, 128), 1, v_scale)
+    return kwargs, want, q_ref, kn
+
+
+def check_q(got, want, dtype):
+    if dtype == torch.bfloat16:
+        ulps = wan_prep.bf16_ulp_distance(got.cpu(), want)
+        assert int(ulps.max()) <= 1 or float((ulps > 1).float().mean()) < 1e-3
+        assert float((ulps > 0).float().mean()) <= 1e-3
+    else:  # the fp32 sum's order: a few 2^-24 of the row's size
+        err = (got.cpu().double() - want.double()).abs().max()
+        assert float(err) <= 2 ** -20 * float(want.double().abs().max())
+
+
+APPENDS = [
+    # streams, grid, frames, heads, kv_heads, page_rows, dtype, ring frames
+    (1, 1, 1, 1, 1, 1, 16, torch.bfloat16, 1),          # one token, one head
+    (3, 1, 1, 1, 12, 12, 128, torch.bfloat16, 5),       # a decoding step
+    (2, 5, 7, 2, 12, 12, 16, torch.bfloat16, 3),        # ring wraps; frames end inside a page
+    (2, 5, 7, 2, 12, 4, 32, torch.bfloat16, 2),         # shared K/V heads
+    (1, 6, 8, 1, 40, 40, 64, torch.bfloat16, 2),        # several warps a token
+    (2, 3, 5, 1, 7, 7, 16, torch.bfloat16, 2),          # an odd number of heads
+    (1, 3, 5, 1, 5, 1, 16, torch.bfloat16, 2),
+    (1, 2, 3, 1, 120, 120, 16, torch.bfloat16, 2),      # the most heads
+    (1, 2, 3, 1, 3, 9, 16, torch.bfloat16, 2),          # more K/V heads than query heads
+    (2, 5, 7, 1, 12, 12, 16, torch.float32, 2),
+    (1, 3, 5, 1, 20, 5, 128, torch.float32, 2),
+    (1, 1, 3, 1, 80, 80, 16, torch.float32, 2),
+]
+
+
+@pytest.mark.parametrize("case", APPENDS)
+@pytest.mark.parametrize("fused", [False, True])
+def test_append_matches_the_definition_bit_for_bit(case, fused):
+    streams, gh, gw, frames, heads, hk, page_rows, dtype, ring = case
+    kwargs, want, q_ref, _ = append_case(*case, seed=heads * 100 + gh, fused=fused)
+    ops.kv4_counters()
+    ops.qk_norm_rope_kv4(**kwargs)
+    assert torch.equal(kwargs["pages"].cpu(), want)     # rows of other slots and spare pages untouched too
+    check_q(kwargs["q_out"], q_ref, dtype)
+    assert ops.kv4_counters() == (0, 0, 0)
+
+
+@pytest.mark.parametrize("k_scale,v_scale,size", [(0.37, 1.7, 1.0), (1e-3, 2.0 ** -20, 30.0), (1e4, 1e6, 1.0),
+                                                  (1e-20, 1e20, 1.0)])
+def test_append_tensor_scales(k_scale, v_scale, size):
+    """Scales that leave blocks saturated, subnormal or zero."""
+    kwargs, want, _, _ = append_case(2, 3, 5, 1, 4, 4, 16, torch.bfloat16, 2, seed=5, k_scale=k_scale, v_scale=v_scale,
+                                     size=size)
+    ops.qk_norm_rope_kv4(**kwargs)
+    assert torch.equal(kwargs["pages"].cpu(), want)
+
+
+def test_append_unaligned_rows_fp32_weights_and_token_tables():
+    """Rows on 16-byte but not 32-byte boundaries take the narrow loads; weights in fp32; explicit tables."""
+    kwargs, want, q_ref, _ = append_case(2, 3, 5, 1, 12, 12, 16, torch.bfloat16, 2, seed=9, w32=True, mode="tokens")
+    T, C = kwargs["q"].shape
+    for name in ("q", "k", "v", "q_out"):
+        wide = torch.empty(T, C + 8, dtype=torch.bfloat16, device=DEV)
+        view = wide[:, 8:]
+        assert view.data_ptr() % 32 == 16
+        view.copy_(kwargs[name])
+        kwargs[name] = view
+    ops.qk_norm_rope_kv4(**kwargs)
+    assert torch.equal(kwargs["pages"].cpu(), want)
+    check_q(kwargs["q_out"], q_ref, torch.bfloat16)
+
+
+def test_append_more_sequences_than_one_launch():
+    case = (70, 1, 3, 1, 2, 2, 16, torch.bfloat16, 2)
+    kwargs, want, q_ref, _ = append_case(*case, seed=3)
+    ops.qk_norm_rope_kv4(**kwargs)
+    assert torch.equal(kwargs["pages"].cpu(), want)
+    check_q(kwargs["q_out"], q_ref, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_append_non_finite_and_zero_inputs(dtype):
+    """V with NaN (stored as zero), infinities (saturate) and zero blocks; each block with one counts."""
+    kwargs, want, _, _ = append_case(1, 4, 4, 1, 2, 2, 16, dtype, 1, seed=8)
+    v = kwargs["v"].cpu()
+    v[0, :16] = 0.0
+    v[1, 3] = float("nan")
+    v[2, 20], v[2, 21] = float("inf"), -float("inf")
+    v[3, 40], v[3, 41] = float("nan"), float("-inf")
+    kwargs["v"] = v.to(DEV)
+    flat = torch.arange(16)
+    table = kwargs["table"].cpu()
+    kv4.store(want, table, flat, v.view(16, 2, 128), 1, kwargs["v_scale"])
+    ops.kv4_counters()
+    ops.qk_norm_rope_kv4(**kwargs)
+    assert torch.equal(kwargs["pages"].cpu(), want)
+    assert ops.kv4_counters().nonfinite == 3
+    back = ops.read_kv4(kwargs["pages"], kwargs["table"], 16, v_scale=kwargs["v_scale"])[1].cpu()
+    assert bool(torch.isfinite(back).all()) and not back[0, 0, :16].any() and back[0, 1, 3] == 0
+
+
+def test_append_nan_in_k_normalises_to_nan_as_the_ring_does():
+    """A NaN in a K row makes RMSNorm's whole row NaN: stored as zeros, k_pre holds the NaN."""
+    kwargs, want, _, kn = append_case(1, 2, 2, 1, 12, 12, 16, torch.bfloat16, 1, seed=8)
+    kwargs["k"][1, 5] = float("nan")
+    kwargs["k_pre"] = torch.empty_like(kwargs["k"])
+    ops.kv4_counters()
+    ops.qk_norm_rope_kv4(**kwargs)
+    assert ops.kv4_counters().nonfinite == 12 * 8
+    assert bool(kwargs["k_pre"][1].isnan().all()) and torch.equal(kwargs["k_pre"][[0, 2, 3]].cpu(), kn[[0, 2, 3]])
+    k, _ = ops.read_kv4(kwargs["pages"], kwargs["table"], 4)
+    assert not k[0, 1].any() and bool(k[0, [0, 2, 3]].any(-1).all())
+
+
+def test_append_roles_and_sinks():
+    """V alone, K alone without a norm, Q alone, and sink rows beside a chunk in one launch."""
+    kwargs, want, q_ref, kn = append_case(1, 3, 4, 1, 4, 4, 16, torch.bfloat16, 3, seed=21)
+    base = {x: kwargs[x] for x in ("heads", "seqs", "cos", "sin", "table", "k_scale", "v_scale")}
+    start = want.clone().zero_()
+    pages = start.to(DEV)
+    ops.qk_norm_rope_kv4(**base, pages=pages, v=kwargs["v"])
+    assert torch.equal(kv4.split(pages.cpu())[0][:, :, 0], kv4.split(start)[0][:, :, 0])
+    ops.qk_norm_rope_kv4(**base, pages=pages, k=kwargs["k"], k_weight=kwargs["k_weight"])
+    rows = kv4.place(kwargs["table"].cpu(), torch.arange(12) + kwargs["seqs"][0].ring_slot0 * 12, 16)
+    for got, ref in zip(kv4.split(pages.cpu()), kv4.split(want)):
+        assert torch.equal(got[rows[0], :, :, rows[1]], ref[rows[0], :, :, rows[1]])
+    q_out = torch.empty_like(kwargs["q"])
+    ops.qk_norm_rope_kv4(**base, pages=pages, q=kwargs["q"], q_weight=kwargs["q_weight"], q_out=q_out)
+    check_q(q_out, q_ref, torch.bfloat16)
+
+    # A sink beside the chunk: its pre-RoPE rows, rotated at frame 9, into the ring's other slot.
+    slot = (kwargs["seqs"][0].ring_slot0 + 1) % 3
+    both = ops.kv4_pages(want.shape[0], 4, 16, DEV)
+    sink = ops.Seq(0, 12, 3, 4, 9, 0, 0, 3, slot, ops.SEQ_SINK)
+    args = {**kwargs, "pages": both, "seqs": [kwargs["seqs"][0], sink], "k_sink": kn.to(DEV)}
+    ops.qk_norm_rope_kv4(**args)
+    c, s = (t for t in wan_prep.frames_table(kwargs["cos"].cpu(), kwargs["sin"].cpu(), wan_prep.axis_dims(128), 9, 10, 3, 4))
+    rot = wan_prep.rope(kn.view(1, 12, 4, 128), c, s)[0]
+    ref = torch.zeros_like(want)
+    kv4.store(ref, kwargs["table"].cpu(), torch.arange(12) + slot * 12, rot, 0, 1.0)
+    place = kv4.place(kwargs["table"].cpu(), torch.arange(12) + slot * 12, 16)
+    for got, r in zip(kv4.split(both.cpu()), kv4.split(ref)):
+        assert torch.equal(got[place[0], :, 0, place[1]], r[place[0], :, 0, place[1]])
+        assert not got[place[0], :, 1, place[1]].any()     # a sink writes no V
+
+
+def test_append_bad_pages_are_skipped_and_counted():
+    kwargs, want, _, _ = append_case(1, 4, 8, 1, 3, 3, 16, torch.bfloat16, 1, seed=30)
+    before = kwargs["pages"].cpu()
+    table = kwargs["table"].cpu()
+    lost = int(table[0, 0])
+    table[0, 0] = want.shape[0]
+    kwargs["table"] = table.to(DEV)
+    ops.kv4_counters()
+    ops.qk_norm_rope_kv4(**kwargs)
+    got = kwargs["pages"].cpu()
+    assert torch.equal(got[lost], before[lost])
+    keep = [p for p in range(want.shape[0]) if p != lost]
+    assert torch.equal(got[keep], want[keep])
+    assert ops.kv4_counters().bad_pages > 0
+    table[0, 0] = -1
+    k, v = ops.read_kv4(kwargs["pages"], table.to(DEV), 32, v_scale=kwargs["v_scale"])
+    assert not k[0, :16].any() and not v[0, :16].any() and bool(k[0, 16:].any())
+    assert ops.kv4_counters().bad_pages > 0
+
+
+def test_append_plan_swaps_tensors():
+    case = (2, 3, 5, 1, 4, 4, 16, torch.bfloat16, 2)
+    kwargs, _, _, _ = append_case(*case, seed=1)
+    other, want, q_ref, _ = append_case(*case, seed=1, size=2.0)
+    kwargs["pages"].copy_(other["pages"])
+    plan = ops.Prep4Plan(**kwargs)
+    plan.launch(q=other["q"], k=other["k"], v=other["v"], q_weight=other["q_weight"], k_weight=other["k_weight"])
+    assert torch.equal(kwargs["pages"].cpu(), want)
+    check_q(kwargs["q_out"], q_ref, torch.bfloat16)
+    with pytest.raises(ops.PrepError, match="swapped"):
+        plan.launch(pages=kwargs["pages"])
+    with pytest.raises(ops.PrepError, match="match"):
+        plan.launch(q=kwargs["q"].float())
+
+
+# ---------------------------------------------------------------------------------------
+# Read
+# ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("members,rows,heads,page_rows,row0,tokens", [
+    (1, 1, 1, 16, 0, 1), (2, 300, 3, 16, 0, 300), (3, 200, 5, 32, 41, 159), (2, 257, 2, 64, 63, 2), (1, 700, 12, 128, 127, 573),
+    (2, 40, 2, 128, 7, 0),
+])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_read_returns_what_the_cache_stands_for(members, rows, heads, page_rows, row0, tokens, dtype):
+    k_scale, v_scale = 0.37, 1.0
+    pages, table, k, v = fill(members, rows, heads, page_rows, rows, k_scale, v_scale)
+    got = ops.read_kv4(pages.to(DEV), table.to(DEV), tokens, row0=row0, k_scale=k_scale, v_scale=v_scale, dtype=dtype)
+    half = 2.0 ** (-8 if dtype == torch.bfloat16 else -24)
+    for x, want in zip(got, (k, v)):
+        assert x.shape == (members, tokens, heads * 128) and x.dtype == dtype
+        want = want[:, row0:row0 + tokens].flatten(2)
+        assert bool(((x.cpu().double() - want).abs() <= half * want.abs()).all())
+    if not tokens:
+        return
+    # Into the caller's strided rows, on 16-byte boundaries only.
+    wide = torch.full((members, tokens + 1, heads * 128 + 8), 7.0, dtype=dtype, device=DEV)
+    out = wide[:, :tokens, 8:]
+    ops.read_kv4(pages.to(DEV), table.to(DEV), tokens, row0=row0, k_scale=k_scale, v_scale=v_scale, k_out=out)
+    assert torch.equal(out, got[0])
+    assert bool((wide[:, tokens] == 7).all()) and bool((wide[..., :8] == 7).all())
+
+
+def test_read_refuses_rows_behind_the_table():
+    pages, table, _, _ = fill(1, 20, 1, 16, 1, extra_pages=0)
+    with pytest.raises(ops.PrepError, match="BOUNDS"):
+        ops.read_kv4(pages.to(DEV), table.to(DEV), 33)
+
+
+# ---------------------------------------------------------------------------------------
+# Attention
+# ---------------------------------------------------------------------------------------
+def check_attention(got, q, k, v, lens, heads, causal_block=0, scale=None, absent=None):
+    want, size = kv4.attention(q, k, v, lens, heads, causal_block, scale, absent)
+    got = got.cpu().double().view(want.shape)
+    top = v.abs().amax(dim=(1, 2, 3))[:, None, None, None] if v.shape[1] else torch.zeros(v.shape[0], 1, 1, 1)
+    bound = 2 ** -8 * want.abs() + 2 ** -10 * size + 2 ** -24 * k.shape[1] * top
+    err = (got - want).abs()
+    worst = float((err / bound.clamp_min(1e-300)).max()) if err.numel() else 0.0
+    assert bool(torch.isfinite(got).all())
+    assert bool((err <= bound).all()), f"{worst:.2f} x the bound, error {float(err.max()):.3e}"
+
+
+ATTENDS = [
+    # members, Lq, heads, kv_heads, page_rows, rows, causal block
+    (1, 1, 1, 1, 16, 1, 0),
+    (1, 1, 12, 12, 128, 257, 0),
+    (3, 1, 4, 4, 16, 100, 0),
+    (2, 3, 8, 2, 16, 300, 1),         # shared heads, causal
+    (2, 5, 4, 2, 32, 129, 0),
+    (1, 8, 2, 2, 64, 128, 0),         # the eight rows of one block
+    (1, 9, 2, 2, 64, 640, 1),
+    (2, 17, 4, 1, 128, 1000, 4),      # several row blocks, blocks of four tokens
+    (1, 40, 3, 3, 32, 33, 1),         # more query rows than window rows: rows that see nothing
+    (2, 130, 2, 1, 16, 390, 30),      # frames of 30, the first query frame sees the past only
+    (1, 300, 2, 2, 128, 1200, 0),
+    (1, 257, 1, 1, 16, 1, 0),
+    (1, 600, 2, 1, 64, 600, 100),
+]
+
+
+@pytest.mark.parametrize("kernel", ["auto", "rows"])
+@pytest.mark.parametrize("chunks", [0, 1, 3])
+@pytest.mark.parametrize("case", ATTENDS)
+def test_attention_matches_64_bits(case, chunks, kernel):
+    members, Lq, heads, hk, page_rows, rows, cb = case
+    pages, table, k, v = fill(members, rows, hk, page_rows, Lq + rows, 0.7, 0.375)
+    q = (torch.randn(members, Lq, heads * 128, generator=gen(rows)) * 1.5).bfloat16()
+    ops.kv4_counters()
+    got = ops.attention_kv4(q.to(DEV), pages.to(DEV), table.to(DEV), rows, heads=heads, k_scale=0.7, v_scale=0.375,
+                            causal_block=cb, key_chunks=chunks, kernel=kernel)
+    assert got.shape == q.shape and got.dtype == torch.bfloat16
+    check_attention(got, q, k, v, [rows] * members, heads, cb)
+    assert ops.kv4_counters() == (0, 0, 0)
+
+
+@pytest.mark.parametrize("kernel", ["auto", "rows"])
+@pytest.mark.parametrize("Lq,cb,chunks", [(1, 0, 0), (3, 1, 4), (200, 0, 2), (200, 60, 0)])
+def test_attention_ragged_lengths(Lq, cb, chunks, kernel):
+    """Lengths on the device: zero, one, inside a page, inside a tile, the whole table, beyond it (clamped)."""
+    lens = [0, 1, 37, 130, 256, 500, 9999, -5]
+    pages, table, k, v = fill(len(lens), 512, 2, 32, 77, extra_pages=0)
+    q = torch.randn(len(lens), Lq, 4 * 128, generator=gen(1)).bfloat16()
+    got = ops.attention_kv4(q.to(DEV), pages.to(DEV), table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV), heads=4,
+                            causal_block=cb, key_chunks=chunks, kernel=kernel)
+    check_attention(got, q, k, v, [min(max(n, 0), 512) for n in lens], 4, cb)
+    assert not got[0].any() and not got[7].any()
+    short = ops.attention_kv4(q.to(DEV), pages.to(DEV), table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV), heads=4,
+                              causal_block=cb, key_chunks=chunks, kernel=kernel, max_kv_tokens=300)
+    check_attention(short, q, k, v, [min(max(n, 0), 300) for n in lens], 4, cb)
+
+
+@pytest.mark.parametrize("kernel", ["auto", "rows"])
+@pytest.mark.parametrize("Lq", [1, 200])
+def test_attention_never_reads_behind_the_window(Lq, kernel):
+    """Table entries behind the window name no page, unwritten rows hold 0xff: neither shows, none is counted."""
+    rows = 70
+    pages, table, k, v = fill(2, rows, 2, 16, 5, extra_pages=4)
+    table[:, 5:] = 1 << 30
+    q = torch.randn(2, Lq, 2 * 128, generator=gen(2)).bfloat16()
+    ops.kv4_counters()
+    for cb in (0, 1):
+        got = ops.attention_kv4(q.to(DEV), pages.to(DEV), table.to(DEV), rows, heads=2, causal_block=cb, kernel=kernel)
+        check_attention(got, q, k, v, [rows] * 2, 2, cb)
+    assert ops.kv4_counters() == (0, 0, 0)
+
+
+@pytest.mark.parametrize("kernel", ["auto", "rows"])
+@pytest.mark.parametrize("Lq,page_rows", [(1, 16), (2, 128), (150, 32), (150, 128)])
+def test_attention_leaves_bad_pages_out(Lq, page_rows, kernel):
+    rows = 500
+    pages, table, k, v = fill(2, rows, 2, page_rows, 6)
+    table[0, 1], table[1, 2] = -1, pages.shape[0]
+    absent = torch.zeros(2, rows, dtype=torch.bool)
+    absent[0, page_rows:2 * page_rows] = True
+    absent[1, 2 * page_rows:3 * page_rows] = True
+    q = torch.randn(2, Lq, 4 * 128, generator=gen(3)).bfloat16()
+    ops.kv4_counters()
+    got = ops.attention_kv4(q.to(DEV), pages.to(DEV), table.to(DEV), rows, heads=4, kernel=kernel)
+    check_attention(got, q, k, v, [rows] * 2, 4, absent=absent)
+    assert ops.kv4_counters().bad_pages > 0
+    table[:] = -7
+    got = ops.attention_kv4(q.to(DEV), pages.to(DEV), table.to(DEV), rows, heads=4, kernel=kernel)
+    assert not got.any()
+    ops.kv4_counters()
+
+
+@pytest.mark.parametrize("kernel", ["auto", "rows"])
+@pytest.mark.parametrize("Lq", [1, 300])
+def test_attention_scores_that_grow_along_the_window(Lq, kernel):
+    """The running reference has to move many times, by far more than 2^8."""
+    rows = 1500
+    pages, table, k, v = fill(1, rows, 2, 64, 9)
+    flat = torch.arange(rows)
+    x = k[0] * torch.linspace(0.1, 8.0, rows, dtype=torch.float64)[:, None, None]
+    kv4.store(pages, table, flat, x.float(), 0, 1.0)
+    k = kv4.load(pages, table, flat, 0, 1.0)[None]
+    q = (torch.randn(1, Lq, 2 * 128, generator=gen(4)) * 4).bfloat16()
+    for chunks in (1, 3):
+        got = ops.attention_kv4(q.to(DEV), pages.to(DEV), table.to(DEV), rows, heads=2, key_chunks=chunks, kernel=kernel)
+        check_attention(got, q, k, v, [rows], 2)
+
+
+@pytest.mark.parametrize("kernel", ["auto", "rows"])
+@pytest.mark.parametrize("Lq", [2, 140])
+@pytest.mark.parametrize("size", [2.0 ** -100, 2.0 ** -14, 1e4, 2.0 ** 80, 0.0])
+def test_attention_query_rows_of_any_size(size, Lq, kernel):
+    """Rows far outside fp16's range, with the scale that brings the scores back."""
+    pages, table, k, v = fill(1, 200, 2, 16, 10)
+    q = (torch.randn(1, Lq, 2 * 128, generator=gen(5)) * size).bfloat16()
+    scale = 0.1 / size if size else None
+    got = ops.attention_kv4(q.to(DEV), pages.to(DEV), table.to(DEV), 200, heads=2, scale=scale, kernel=kernel)
+    check_attention(got, q, k, v, [200], 2, scale=scale)
+
+
+@pytest.mark.parametrize("kernel", ["auto", "rows"])
+@pytest.mark.parametrize("Lq", [3, 140])
+def test_attention_non_finite_queries_stay_in_their_rows(Lq, kernel):
+    pages, table, k, v = fill(1, 300, 2, 128, 12)
+    q = torch.randn(1, Lq, 2 * 128, generator=gen(6)).bfloat16()
+    clean = ops.attention_kv4(q.to(DEV), pages.to(DEV), table.to(DEV), 300, heads=2, kernel=kernel)
+    q[0, 1, 7] = float("nan")          # head 0
+    q[0, 2, 128 + 9] = float("inf")    # head 1
+    got = ops.attention_kv4(q.to(DEV), pages.to(DEV), table.to(DEV), 300, heads=2, kernel=kernel)
+    assert bool(got[0, 1, :128].isnan().all()) and bool(got[0, 2, 128:].isnan().all())
+    got[0, 1, :128], got[0, 2, 128:] = clean[0, 1, :128], clean[0, 2, 128:]
+    assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("kernel", ["auto", "rows"])
+@pytest.mark.parametrize("Lq", [2, 150])
+def test_attention_strides_and_outputs_in_place(Lq, kernel):
+    """Q as [B, L, H, D] out of a wider buffer, the output into a wider one; nothing beside it is written."""
+    pages, table, k, v = fill(2, 300, 2, 32, 13)
+    buf = torch.randn(2, Lq + 3, 4 * 128 + 64, generator=gen(7)).bfloat16()
+    q = buf[:, 1:Lq + 1, 32:32 + 512]
+    wide = torch.full((2, Lq + 2, 640), 5.0, dtype=torch.bfloat16, device=DEV)
+    out = wide[:, :Lq, 64:576]
+    dev = buf.to(DEV)[:, 1:Lq + 1, 32:32 + 512].unflatten(2, (4, 128))
+    got = ops.attention_kv4(dev, pages.to(DEV), table.to(DEV), 300, heads=4, out=out, kernel=kernel)
+    assert got is out
+    check_attention(out, q, k, v, [300] * 2, 4)
+    assert bool((wide[:, Lq:] == 5).all()) and bool((wide[..., :64] == 5).all()) and bool((wide[..., 576:] == 5).all())
+
+
+@pytest.mark.parametrize("Lq", [1, 200])
+def test_attention_replays_from_a_graph_with_new_lengths(Lq):
+    """One captured call: the lengths, pages and queries are read at replay."""
+    pages, table, k, v = fill(2, 700, 2, 16, 14)
+    q = torch.randn(2, Lq, 4 * 128, generator=gen(8)).bfloat16()
+    dq, dp, dt = q.to(DEV), pages.to(DEV), table.to(DEV)
+    lens = torch.tensor([700, 700], dtype=torch.int32, device=DEV)
+    ops.attention_kv4(dq, dp, dt, lens, heads=4)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.attention_kv4(dq, dp, dt, lens, heads=4)
+    for ns in ([5, 640], [0, 129], [700, 1]):
+        lens.copy_(torch.tensor(ns, dtype=torch.int32))
+        graph.replay()
+        check_attention(out, q, k, v, ns, 4)
+
+
+def test_two_graphs_and_an_eager_call_do_not_share_partial_results():
+    """Calls on two streams at once: each has its own workspace."""
+    pages, table, k, v = fill(1, 3000, 2, 128, 15)
+    dp, dt = pages.to(DEV), table.to(DEV)
+    qs = [torch.randn(1, 2, 2 * 128, generator=gen(20 + i)).bfloat16() for i in range(3)]
+    dq = [q.to(DEV) for q in qs]
+    graphs, outs = [], []
+    for i in range(2):
+        ops.attention_kv4(dq[i], dp, dt, 3000, heads=2, key_chunks=8)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            outs.append(ops.attention_kv4(dq[i], dp, dt, 3000, heads=2, key_chunks=8))
+    side = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, s in zip(graphs, side):
+            with torch.cuda.stream(s):
+                g.replay()
+        eager = ops.attention_kv4(dq[2], dp, dt, 3000, heads=2, key_chunks=8)
+    torch.cuda.synchronize()
+    for out, q in zip((*outs, eager), qs):
+        check_attention(out, q, k, v, [3000], 2)
+
+
+def test_results_do_not_depend_on_the_run():
+    pages, table, _, _ = fill(2, 2000, 2, 64, 16)
+    for Lq in (1, 300):
+        q = torch.randn(2, Lq, 4 * 128, generator=gen(9)).bfloat16().to(DEV)
+        runs = [ops.attention_kv4(q, pages.to(DEV), table.to(DEV), 2000, heads=4) for _ in range(3)]
+        assert torch.equal(runs[0], runs[1]) and torch.equal(runs[0], runs[2])
+
+
+def test_attention_refusals():
+    pages, table, _, _ = fill(2, 50, 2, 16, 17)
+    dp, dt = pages.to(DEV), table.to(DEV)
+    q = torch.zeros(2, 3, 512, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ops.PrepError, match="bfloat16"):
+        ops.attention_kv4(q.float(), dp, dt, 50, heads=4)
+    with pytest.raises(ops.PrepError):
+        ops.attention_kv4(q, dp, dt, 50, heads=3)
+    with pytest.raises(ops.PrepError):
+        ops.attention_kv4(q[:1], dp, dt, 50, heads=4)
+    with pytest.raises(ops.PrepError, match="outside"):
+        ops.attention_kv4(q, dp, dt, 81, heads=4)
+    with pytest.raises(ops.PrepError, match="int32"):
+        ops.attention_kv4(q, dp, dt, torch.zeros(2, device=DEV), heads=4)
+    with pytest.raises(ops.PrepError, match="out"):
+        ops.attention_kv4(q, dp, dt, 50, heads=4, out=torch.empty(2, 4, 512, dtype=torch.bfloat16, device=DEV))
+    with pytest.raises(ops.PrepError, match="kernel"):
+        ops.attention_kv4(q, dp, dt, 50, heads=4, kernel="fast")
+    assert ops.attention_kv4(q[:, :0], dp, dt, 50, heads=4).shape == (2, 0, 512)
+
+
+def test_offsets_beyond_32_bits():
+    """A pool of over 4 GiB: the last pages are written and read where they are."""
+    heads, page_rows = 40, 128
+    page_bytes = heads * 2 * page_rows * 72
+    n = (1 << 32) // page_bytes + 5
+    pages = torch.zeros(n, heads, 2, page_rows * 72, dtype=torch.uint8, device=DEV)
+    table = torch.tensor([[n - 1, 3, n - 2]], dtype=torch.int32)
+    g = gen(1)
+    x = torch.randn(300, heads * 128, generator=g).bfloat16()
+    seqs = [ops.Seq(0, 300, 1, 300, 0, 0, 0, 1, 0)]
+    ops.qk_norm_rope_kv4(heads=heads, seqs=seqs, v=x.to(DEV), pages=pages, table=table.to(DEV))
+    _, v = ops.read_kv4(pages, table.to(DEV), 300)
+    ref = torch.zeros(3, heads, 2, page_rows * 72, dtype=torch.uint8)
+    small = torch.tensor([[0, 1, 2]], dtype=torch.int32)
+    kv4.store(ref, small, torch.arange(300), x.view(300, heads, 128), 1, 1.0)
+    want = kv4.load(ref, small, torch.arange(300), 1, 1.0)
+    assert torch.equal(v.cpu().double().view(300, heads, 128), want)
+    q = torch.randn(1, 1, heads * 128, generator=g).bfloat16()
+    k = torch.zeros(1, 300, heads, 128, dtype=torch.float64)
+    check_attention(ops.attention_kv4(q.to(DEV), pages, table.to(DEV), 300, heads=heads), q, k, want[None], [300], heads)
