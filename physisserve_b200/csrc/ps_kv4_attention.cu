@@ -8,6 +8,7 @@
 #include <string.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "ps_kv4.cuh"
 #include "ps_sm100.cuh"
@@ -28,12 +29,15 @@ struct AParams {
   int32_t Lq, kv_max, causal_block, group;
   int32_t rows;          // query rows of a K/V head: Lq * group
   int32_t row_blocks;    // blocks of query rows per K/V head
-  int32_t chunks;        // key chunks per unit
-  int32_t grid;          // persistent CTAs (tiles kernel)
+  int32_t chunks;        // rows kernel: key chunks per unit
+  int32_t grid;          // tiles kernel: persistent CTAs
+  int32_t min_steps;     // tiles kernel: fewest steps of a CTA
   int64_t units;         // members * kv_heads * row_blocks
   float scale_log2;      // softmax scale * k_scale * log2(e)
-  float* ws_o;           // [units][chunks][rows of a block][128] unnormalised sums (chunks > 1)
-  float2* ws_ml;         // [units][chunks][rows of a block] (reference in log2 units, sum)
+  float* ws_o;           // partial results: [slots][rows of a block][128] unnormalised sums,
+  float2* ws_ml;         // [slots][rows of a block] (reference in log2 units, sum); slots are
+                         // [units][chunks] (rows kernel) or [grid][2] (tiles kernel)
+  int4* ws_units;        // tiles kernel: [units] (first CTA, last CTA, the first CTA's slot, 0)
 };
 
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int* abort_flag, bool count = true) {
@@ -502,6 +506,616 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const __grid_constant_
 }
 
 // ---------------------------------------------------------------------------------------
+// tiles kernel: 256 query rows of a K/V head at a time, tcgen05
+// ---------------------------------------------------------------------------------------
+// Bound: the tensor cores (4 * 128 * 256 flops a key), with the 16 exponentials a clock of an SM's
+// special-function unit next (256 of them a key: as many clocks as the products take).
+//
+// A unit is (member, K/V head, 256 query rows) = two 128-row query tiles that share every K/V tile.
+// Its work is the 128-key tiles that any of its rows sees ("steps").  The steps of all units, in
+// order, are cut into equal contiguous ranges, one per CTA, one CTA per SM: every SM gets the same
+// number of steps whatever the windows' lengths and masks are, and at most the first and the last unit
+// of a range are shared with a neighbour.  Those leave partial results (unnormalised O, reference,
+// sum) in two workspace slots per CTA; kv4_merge_kernel joins them.
+//
+// CTA of four warpgroups:
+//   warps 0-3    dequantise: each thread reads 16 bytes (32 elements) of four keys of K, then of V, one
+//                tile ahead in registers, and writes them as fp16 into the 128-byte swizzled tiles that the
+//                tensor core reads.  The packed bytes come from L2 or HBM straight into registers: a
+//                tile of K and V is 18 KB where it would be 64 KB in bf16;
+//   warps 4-7    softmax of query tile 0, warps 8-11 of tile 1: a query row per thread (TMEM lane = row);
+//                they also bring the row's Q, scaled to fp16, into shared memory;
+//   warp 12      owns the tensor memory (512 columns: O0 | S0 | O1 | S1) and issues the MMAs in the order
+//                PV0(t), S0(t+1), PV1(t), S1(t+1), so that one tile's products run under the other's
+//                exponentials.  P overwrites the S columns that were read; P V starts on the first half of
+//                the keys while the second half is exponentiated.
+// tcgen05.mma operations of one thread complete in issue order, so a commit after S_i(t+1) also reports
+// P_i(t) V(t) done.  All waits are bounded: one that runs out raises the CTA's abort flag, every role
+// leaves its loop, the MMA warp waits for its MMAs and frees the tensor memory.
+constexpr int kM = 128;
+constexpr int kUnitRows = 2 * kM;
+constexpr int kTile16 = kM * kKv4D * 2;    // bytes of a 128 x 128 fp16 tile
+constexpr int kHalf16 = kTile16 / 2;       // its 64-column half
+constexpr int kTilesThreads = 512;
+constexpr int kDequantRegs = 96, kSoftmaxRegs = 184, kMmaRegs = 48;
+static_assert(kDequantRegs + 2 * kSoftmaxRegs + kMmaRegs <= 512, "register split exceeds the launch's 128 a thread");
+constexpr int kOffQ = 0, kOffK = kOffQ + 2 * kTile16, kOffV = kOffK + 2 * kTile16, kOffBars = kOffV + 2 * kTile16;
+enum TBar {
+  kQFull, kKFull = kQFull + 2, kKEmpty = kKFull + 2, kVFull = kKEmpty + 2, kVEmpty = kVFull + 2, kSFull = kVEmpty + 2,
+  kPHalf = kSFull + 2, kPFull = kPHalf + 2, kOFinal = kPFull + 2, kMmaDone = kOFinal + 2, kTBars
+};
+constexpr int kOffTmem = kOffBars + 8 * kTBars, kOffAbort = kOffTmem + 4, kOffStart = kOffAbort + 4;
+constexpr int kTilesSmem = kOffStart + 32 + 1024;
+static_assert(kTilesSmem <= 227 * 1024, "tiles exceed shared memory");
+__host__ __device__ constexpr int col_o(int i) { return 256 * i; }
+__host__ __device__ constexpr int col_s(int i) { return 256 * i + 128; }
+// kind::f16 with fp16 operands, fp32 accumulators, M = N = 128; b_mn: B's N runs along its rows.
+__host__ __device__ constexpr uint32_t idesc16(uint32_t b_mn) {
+  return (1u << 4) | (b_mn << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+template <int N> __device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N> __device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+// wait_bar inline: the register splits above do not survive a call.
+__device__ __forceinline__ bool spin_bar(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  if (bar_test(bar, parity)) return true;
+  const unsigned long long start = now_ns();
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i)
+      if (bar_try(bar, parity)) return true;
+    if (*abort_flag) return false;
+    if (now_ns() - start > kBarWaitNs) {
+      atomicAdd(&g_kv4_counts[kKv4Timeouts], 1u);
+      *abort_flag = 1;
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ bool warp_spin(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, spin_bar(bar, parity, abort_flag));
+}
+
+// Steps of a unit of member b with n window rows: the 128-key tiles that any of its rows sees, at least
+// one (a unit that sees nothing still has zeros to write).
+__device__ __forceinline__ int unit_steps(const AParams& p, int n, int qb, int& lim_top) {
+  const int last = min((qb + 1) * kUnitRows, p.rows) - 1;
+  lim_top = token_limit(p, n, last / p.group);
+  return max(1, (lim_top + kTileKeys - 1) / kTileKeys);
+}
+
+// A CTA's way through its range of steps; every role walks the same way.
+struct Walk {
+  int b, h, qb, n, lim_top;
+  int j0, j1;        // key tiles of the present segment
+  int steps;         // steps of the present unit
+  int64_t at, end;   // step of j0, end of the CTA's range
+  bool first;        // the CTA's first segment
+
+  __device__ __forceinline__ bool begin(const AParams& p, const int4& start, int64_t s0, int64_t s1) {
+    b = start.x;
+    h = start.y;
+    qb = start.z;
+    j0 = start.w;
+    at = s0;
+    end = s1;
+    first = true;
+    return at < end && (open(p), true);
+  }
+  __device__ __forceinline__ void open(const AParams& p) {
+    n = member_len(p, b);
+    steps = unit_steps(p, n, qb, lim_top);
+    j1 = static_cast<int>(min(static_cast<int64_t>(steps), j0 + (end - at)));
+  }
+  __device__ __forceinline__ bool next(const AParams& p) {
+    at += j1 - j0;
+    if (at >= end) return false;
+    first = false;
+    j0 = 0;
+    if (++qb == p.row_blocks) {
+      qb = 0;
+      if (++h == p.cache.kv_heads) {
+        h = 0;
+        ++b;
+      }
+    }
+    open(p);
+    return true;
+  }
+  __device__ __forceinline__ bool two(const AParams& p) const { return qb * kUnitRows + kM < p.rows; }
+  __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == steps; }
+  __device__ __forceinline__ int64_t unit(const AParams& p) const {
+    return (static_cast<int64_t>(b) * p.cache.kv_heads + h) * p.row_blocks + qb;
+  }
+};
+
+// Total steps, and the unit and tile at which step `per * cta` lies (one warp; `per` is derived from the
+// total).
+__device__ __forceinline__ void find_start(const AParams& p, int64_t members, int lane, int64_t& per, int64_t& total,
+                                           int4& start) {
+  int lim;
+  const int hk = p.cache.kv_heads;
+  if (!p.lens && p.causal_block == 0) {  // every unit has the same number of steps
+    const int steps = unit_steps(p, p.kv_max, 0, lim);
+    total = p.units * steps;
+    per = max((total + p.grid - 1) / p.grid, static_cast<int64_t>(p.min_steps));
+    const int64_t u = per * blockIdx.x / steps;
+    const int64_t bh = u / p.row_blocks;
+    start = make_int4(static_cast<int>(bh / hk), static_cast<int>(bh % hk), static_cast<int>(u % p.row_blocks),
+                      static_cast<int>(per * blockIdx.x % steps));
+    return;
+  }
+  auto member_steps = [&](int b) {
+    const int n = member_len(p, b);
+    int64_t sum = 0;
+    for (int q = lane; q < p.row_blocks; q += 32) sum += unit_steps(p, n, q, lim);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    return sum;
+  };
+  total = 0;
+  for (int b = 0; b < members; ++b) total += hk * member_steps(b);
+  per = max((total + p.grid - 1) / p.grid, static_cast<int64_t>(p.min_steps));
+  int64_t left = per * blockIdx.x;
+  start = make_int4(0, 0, 0, 0);
+  if (left >= total) return;
+  int b = 0;
+  int64_t sum = member_steps(0);
+  while (left >= hk * sum) {
+    left -= hk * sum;
+    sum = member_steps(++b);
+  }
+  const int h = static_cast<int>(left / sum);
+  left -= h * sum;
+  const int n = member_len(p, b);
+  for (int q0 = 0;; q0 += 32) {
+    const int mine = q0 + lane < p.row_blocks ? unit_steps(p, n, q0 + lane, lim) : 0;
+    int64_t upto = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += y;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, upto > left);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      const int64_t before = __shfl_sync(0xffffffffu, upto - mine, l);
+      start = make_int4(b, h, q0 + l, static_cast<int>(left - before));
+      return;
+    }
+    left -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+}
+
+__global__ void __launch_bounds__(kTilesThreads, 1)
+    kv4_tiles_kernel(const __grid_constant__ AParams p, const int64_t members) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = saddr(smem);
+  auto bar = [&](int i) { return sbase + kOffBars + 8u * static_cast<uint32_t>(i); };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kOffAbort);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kOffTmem);
+  int64_t* range = reinterpret_cast<int64_t*>(smem + kOffStart);  // [per, total], then the start
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      bar_init(bar(kQFull + i), 128);
+      bar_init(bar(kKFull + i), 4);
+      bar_init(bar(kKEmpty + i), 1);
+      bar_init(bar(kVFull + i), 4);
+      bar_init(bar(kVEmpty + i), 1);
+      bar_init(bar(kSFull + i), 1);
+      bar_init(bar(kPHalf + i), 128);
+      bar_init(bar(kPFull + i), 128);
+      bar_init(bar(kOFinal + i), 1);
+    }
+    bar_init(bar(kMmaDone), 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(tmem_slot)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait();
+  if (warp == 0) {
+    int64_t per, total;
+    int4 start;
+    find_start(p, members, lane, per, total, start);
+    if (lane == 0) {
+      range[0] = per;
+      range[1] = total;
+      *reinterpret_cast<int4*>(range + 2) = start;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int64_t per = range[0];
+  const int4 start = *reinterpret_cast<int4*>(range + 2);
+  const int64_t s0 = min(per * blockIdx.x, range[1]), s1 = min(s0 + per, range[1]);
+  const int shift = p.cache.shift;
+  Walk w;
+
+  if (warp < 4) {
+    // ------------------------------- dequantisers -------------------------------
+    regs_dec<kDequantRegs>();
+    // Lane (r, c): 16-byte chunk c (elements 32c .. 32c+31) of keys 32 i + 8 warp + r, i = 0..3.  A warp
+    // reads 512 contiguous bytes of 8 keys at a time (their page is one: pages hold 16 rows or more).
+    // Chunks 0 and 1 go to the tile's left half, 2 and 3 to its right one, whose rows fall into the same
+    // banks: lanes of the right half write their four 16-byte parts in the order 2 3 0 1, so that
+    // eight lanes of a store cover all banks.
+    const int r = lane >> 2, c = lane & 3;
+    const bool right = c >= 2;
+    const int half = static_cast<int>(p.cache.head_bytes >> 1);
+    const int page_rows = 1 << shift;
+    uint32_t dst[4];  // byte offset of part i (in write order) of key row 8 warp + r
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int part = (c & 1) * 4 + (right ? i ^ 2 : i);
+      dst[i] = (c >> 1) * kHalf16 + (8 * warp + r) * 128 + ((part ^ r) * 16);
+    }
+    uint4 kw[4], vw[4];
+    uint32_t ks[4], vs[4];
+    int64_t page[4];
+    // Pages of the four keys of tile j; -1 where nothing is to be read.
+    auto pages = [&](int j, bool count) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = j * kTileKeys + 32 * i + 8 * warp + r;
+        page[i] = -1;
+        if (key < w.lim_top) {
+          const int32_t x = p.cache.table[w.b * p.cache.table_pages + (key >> shift)];
+          if (static_cast<uint32_t>(x) < p.cache.num_pages) page[i] = x;
+          else if (count && c == 0 && (key & (page_rows - 1)) == 0) atomicAdd(&g_kv4_counts[kKv4BadPages], 1u);
+        }
+      }
+    };
+    auto load = [&](uint4* x, uint32_t* s, int off) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = make_uint4(0, 0, 0, 0);
+        s[i] = 0;
+        if (page[i] >= 0) {
+          const int in_page = (32 * i + 8 * warp + r) & (page_rows - 1);
+          const unsigned char* base = kv4_head(p.cache, page[i], w.h) + off;
+          x[i] = *reinterpret_cast<const uint4*>(base + in_page * 64 + c * 16);
+          s[i] = *reinterpret_cast<const uint16_t*>(base + page_rows * 64 + in_page * 8 + c * 2);
+        }
+      }
+    };
+    auto expand = [&](const uint4* x, const uint32_t* s, uint32_t tile) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t s2 = kv4_scales(s[i]);
+        const uint32_t sa = __byte_perm(s2, s2, right ? 0x3232 : 0x1010), sb = __byte_perm(s2, s2, right ? 0x1010 : 0x3232);
+        const uint32_t q[4] = {right ? x[i].z : x[i].x, right ? x[i].w : x[i].y, right ? x[i].x : x[i].z,
+                               right ? x[i].y : x[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t o[4];
+          kv4_unpack(q[k], o);
+          const uint32_t sc = k < 2 ? sa : sb;
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(tile + 32 * i * 128 + dst[k]), "r"(h2_mul(o[0], sc)),
+                       "r"(h2_mul(o[1], sc)), "r"(h2_mul(o[2], sc)), "r"(h2_mul(o[3], sc))
+                       : "memory");
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+    };
+    int t = 0;
+    bool ok = true;
+    for (bool more = w.begin(p, start, s0, s1); ok && more; more = w.next(p)) {
+      pages(w.j0, true);
+      load(kw, ks, 0);
+      load(vw, vs, half);
+      for (int j = w.j0; j < w.j1; ++j, ++t) {
+        const int st = t & 1;
+        const uint32_t parity = ((t >> 1) & 1) ^ 1;
+        if (j + 1 < w.j1) pages(j + 1, true);
+        if (t >= 2 && !(ok = warp_spin(bar(kKEmpty + st), parity, abort_flag))) break;
+        expand(kw, ks, sbase + kOffK + st * kTile16);
+        if (lane == 0) bar_arrive(bar(kKFull + st));
+        if (j + 1 < w.j1) load(kw, ks, 0);
+        if (t >= 2 && !(ok = warp_spin(bar(kVEmpty + st), parity, abort_flag))) break;
+        expand(vw, vs, sbase + kOffV + st * kTile16);
+        if (lane == 0) bar_arrive(bar(kVFull + st));
+        if (j + 1 < w.j1) load(vw, vs, half);
+      }
+    }
+  } else if (warp >= 12) {
+    regs_dec<kMmaRegs>();
+    if (warp == 12 && lane == 0) {
+      // ------------------------------- MMA issuer -------------------------------
+      const uint32_t id_s = idesc16(0), id_pv = idesc16(1);
+      const uint64_t qd0 = smem_desc(sbase + kOffQ, 16, 1024), kd0 = smem_desc(sbase + kOffK, 16, 1024);
+      const uint64_t vd0 = smem_desc(sbase + kOffV, kHalf16, 1024);
+      auto issue_s = [&](int i, int t) {
+        const uint64_t qd = qd0 + (i ? kTile16 >> 4 : 0), kd = kd0 + ((t & 1) ? kTile16 >> 4 : 0);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint64_t off = static_cast<uint64_t>(((k >> 2) * kHalf16 + (k & 3) * 32) >> 4);
+          tc_mma(tmem + col_s(i), qd + off, kd + off, id_s, k > 0);
+        }
+      };
+      // Four 16-key steps of P V from step k0.
+      auto issue_pv = [&](int i, int t, int k0, bool fresh) {
+        const uint64_t vd = vd0 + ((t & 1) ? kTile16 >> 4 : 0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          tc_mma_ts(tmem + col_o(i), tmem + col_s(i) + (k0 + k) * 8, vd + static_cast<uint64_t>((k0 + k) * 128), id_pv,
+                    !(fresh && k0 + k == 0));
+      };
+      int t = 0, tq[2] = {0, 0}, segs[2] = {0, 0};  // key tiles; tiles and segments of each query tile
+      bool ok = true;
+      for (bool more_segs = w.begin(p, start, s0, s1); ok && more_segs; more_segs = w.next(p)) {
+        const int nq = w.two(p) ? 2 : 1, count = w.j1 - w.j0;
+        if (!(ok = spin_bar(bar(kKFull + (t & 1)), (t >> 1) & 1, abort_flag))) break;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (i >= nq) continue;
+          if (!(ok = spin_bar(bar(kQFull + i), segs[i] & 1, abort_flag))) break;
+          ++segs[i];
+          tc_fence_after();
+          issue_s(i, t);
+          tc_commit(bar(kSFull + i));
+        }
+        if (!ok) break;
+        tc_commit(bar(kKEmpty + (t & 1)));
+        for (int jj = 0; ok && jj < count; ++jj, ++t) {
+          const bool more = jj + 1 < count;
+          if (!(ok = spin_bar(bar(kVFull + (t & 1)), (t >> 1) & 1, abort_flag))) break;
+          if (more && !(ok = spin_bar(bar(kKFull + ((t + 1) & 1)), ((t + 1) >> 1) & 1, abort_flag))) break;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (i >= nq) continue;
+            if (!(ok = spin_bar(bar(kPHalf + i), tq[i] & 1, abort_flag))) break;
+            tc_fence_after();
+            issue_pv(i, t, 0, jj == 0);
+            if (!(ok = spin_bar(bar(kPFull + i), tq[i] & 1, abort_flag))) break;
+            ++tq[i];
+            tc_fence_after();
+            issue_pv(i, t, 4, false);
+            const bool last = i == nq - 1;
+            if (more) {
+              issue_s(i, t + 1);
+              tc_commit(bar(kSFull + i));
+              if (last) tc_commit(bar(kKEmpty + ((t + 1) & 1)));
+            } else {
+              tc_commit(bar(kOFinal + i));
+            }
+            if (last) tc_commit(bar(kVEmpty + (t & 1)));
+          }
+        }
+      }
+      tc_commit(bar(kMmaDone));
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------- softmax -------------------------------
+    regs_inc<kSoftmaxRegs>();
+    const int qi = (warp - 4) >> 2;
+    const int row = (warp & 3) * 32 + lane;  // row of the query tile = TMEM lane
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t s_addr = lanes + col_s(qi), o_addr = lanes + col_o(qi);
+    const int segs_tile = kTileKeys >> shift;
+    int n_tiles = 0, n_segs = 0;
+    bool ok = true;
+    for (bool more = w.begin(p, start, s0, s1); ok && more; more = w.next(p)) {
+      if (qi == 1 && !w.two(p)) continue;
+      const int q_row = w.qb * kUnitRows + qi * kM + row;  // of the K/V head's rows
+      const int token = min(q_row, p.rows - 1) / p.group;
+      const int lim = token_limit(p, w.n, token);
+      // Rows grow downwards, and so do their limits: the tile's first row sees the fewest keys.
+      const int lim_low = token_limit(p, w.n, min(w.qb * kUnitRows + qi * kM, p.rows - 1) / p.group);
+      const int64_t head_off = static_cast<int64_t>(w.h * p.group + (min(q_row, p.rows - 1) - token * p.group)) * kKv4D;
+      float scale;
+      {
+        // This thread's query row: scaled to fp16 and stored 128-byte swizzled.
+        uint4 x[16];
+        const __nv_bfloat16* src = p.q + w.b * p.q_member + token * p.q_row + head_off;
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          x[i] = q_row < p.rows ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0, 0, 0, 0);
+          top = __vmaxu2(top, __vmaxu2(__vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu),
+                                       __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu)));
+        }
+        float back;
+        const float power = row_power(__uint_as_float(max(top << 16, top & 0xffff0000u)), back);
+        scale = fmaxf(back * p.scale_log2, 1.2e-38f);  // not 0: a masked score times it stays -inf
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+          uint32_t o[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            o[e] = h2_pack(__uint_as_float(v[e] << 16) * power, __uint_as_float(v[e] & 0xffff0000u) * power);
+          const uint32_t dst = sbase + kOffQ + qi * kTile16 + (i >> 3) * kHalf16 + row * 128 + (((i & 7) ^ (row & 7)) * 16);
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3])
+                       : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        tc_fence_before();
+        bar_arrive(bar(kQFull + qi));
+      }
+      float m = -INFINITY, l = 0.f;
+      for (int j = w.j0; j < w.j1; ++j, ++n_tiles) {
+        // Pages of the tile that are not in the pool: their keys are left out.
+        int32_t page = 0;
+        if (lane < segs_tile && j * kTileKeys + (lane << shift) < w.lim_top)
+          page = p.cache.table[w.b * p.cache.table_pages + ((j * kTileKeys) >> shift) + lane];
+        const uint32_t bad = __ballot_sync(0xffffffffu, static_cast<uint32_t>(page) >= p.cache.num_pages);
+        if (!(ok = warp_spin(bar(kSFull + qi), n_tiles & 1, abort_flag))) break;
+        tc_fence_after();
+        uint32_t s[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, s + 32 * c);
+        tmem_wait_ld();
+        if ((j + 1) * kTileKeys > lim_low || bad) {
+          const int valid = lim - j * kTileKeys;
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (i >= valid || ((bad >> (i >> shift)) & 1)) s[i] = __float_as_uint(-INFINITY);
+        }
+        float mx[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx[e] = __uint_as_float(s[e]);
+#pragma unroll
+        for (int i = 8; i < 128; i += 8)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(s[i + e]));
+        const float top =
+            fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))) * scale;
+        // The reference moves only when a score exceeds it by more than 8: P is exact for any reference.
+        const bool grow = top > m + 8.f;
+        const float alpha = grow ? fast_exp2(m - top) : 1.f;
+        if (grow) {
+          l *= alpha;
+          m = top;
+        }
+        // O holds this segment's earlier tiles (their P V have completed: S was committed after them).
+        if (__any_sync(0xffffffffu, grow) && j > w.j0) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + 32 * c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st32(o_addr + 32 * c, o);
+          }
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const float x0 = fast_exp2(fmaf(__uint_as_float(s[32 * h + 2 * c]), scale, -ref));
+            const float x1 = fast_exp2(fmaf(__uint_as_float(s[32 * h + 2 * c + 1]), scale, -ref));
+            ls[(c & 1) * 2] += x0;
+            ls[(c & 1) * 2 + 1] += x1;
+            pk[c] = h2_pack(x0, x1);
+          }
+          tmem_st16(s_addr + 16 * h, pk);
+          if (h & 1) {
+            tmem_wait_st();
+            tc_fence_before();
+            bar_arrive(bar((h == 1 ? kPHalf : kPFull) + qi));
+          }
+        }
+        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+      }
+      if (!ok) break;
+      if (!(ok = warp_spin(bar(kOFinal + qi), n_segs & 1, abort_flag))) break;
+      ++n_segs;
+      tc_fence_after();
+      const bool live = q_row < p.rows;
+      if (w.whole()) {
+        const float inv = l == 0.f ? 0.f : p.cache.v_scale / l;
+        __nv_bfloat16* dst = p.out + w.b * p.out_member + token * p.out_row + head_off;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld32(o_addr + 32 * c, o);
+          tmem_wait_ld();
+          if (live) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              uint32_t y[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                y[e] = l == 0.f ? 0u
+                                : Pairs16<__nv_bfloat16>::pack_pair(__uint_as_float(o[8 * v + 2 * e]) * inv,
+                                                                    __uint_as_float(o[8 * v + 2 * e + 1]) * inv);
+              *reinterpret_cast<uint4*>(dst + 32 * c + 8 * v) = make_uint4(y[0], y[1], y[2], y[3]);
+            }
+          }
+        }
+      } else {
+        const int64_t slot = (2ll * blockIdx.x + (w.first ? 0 : 1)) * kUnitRows + qi * kM + row;
+        float* dst = p.ws_o + slot * kKv4D;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld32(o_addr + 32 * c, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + 32 * c + 8 * v), "r"(o[8 * v]),
+                         "r"(o[8 * v + 1]), "r"(o[8 * v + 2]), "r"(o[8 * v + 3]), "r"(o[8 * v + 4]), "r"(o[8 * v + 5]),
+                         "r"(o[8 * v + 6]), "r"(o[8 * v + 7])
+                         : "memory");
+        }
+        p.ws_ml[slot] = make_float2(m, l);
+      }
+      if (qi == 0 && row == 0 && w.j0 == 0) {
+        const int last = static_cast<int>((w.at + w.steps - 1) / per);
+        p.ws_units[w.unit(p)] = make_int4(static_cast<int>(blockIdx.x), last, w.first ? 0 : 1, 0);
+      }
+      tc_fence_before();
+    }
+  }
+
+  // Teardown: every role has left its loop; wait for the MMAs in flight, free the tensor memory.
+  pdl_trigger();
+  __syncthreads();
+  if (warp == 12) {
+    if (lane == 0) {
+      volatile int never = 0;
+      spin_bar(bar(kMmaDone), 0, &never);
+    }
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+// Merges the segments of the units that several CTAs of the tiles kernel shared.  A warp per query row.
+__global__ void __launch_bounds__(256) kv4_merge_kernel(const __grid_constant__ AParams p) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = blockIdx.x / (kUnitRows / 8);
+  const int r = static_cast<int>(blockIdx.x % (kUnitRows / 8)) * 8 + (threadIdx.x >> 5);
+  const int4 info = p.ws_units[unit];  // first CTA, last CTA, slot of the first CTA
+  if (info.x == info.y) return;
+  const int64_t bh = unit / p.row_blocks;
+  const int row = static_cast<int>(unit - bh * p.row_blocks) * kUnitRows + r;
+  if (row >= p.rows) return;
+  auto slot_of = [&](int cta) { return (2ll * cta + (cta == info.x ? info.z : 0)) * kUnitRows + r; };
+  float top = -INFINITY, sum = 0.f;
+  for (int c = info.x; c <= info.y; ++c) top = fmaxf(top, p.ws_ml[slot_of(c)].x);
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c = info.x; c <= info.y; ++c) {
+    const int64_t slot = slot_of(c);
+    const float2 ml = p.ws_ml[slot];
+    if (ml.y == 0.f) continue;  // the row saw nothing there
+    const float f = ml.x == top ? 1.f : fast_exp2(ml.x - top);
+    const float4 y = *reinterpret_cast<const float4*>(p.ws_o + slot * kKv4D + 4 * lane);
+    sum += f * ml.y;
+    x.x += f * y.x;
+    x.y += f * y.y;
+    x.z += f * y.z;
+    x.w += f * y.w;
+  }
+  const float inv = sum == 0.f ? 0.f : p.cache.v_scale / sum;
+  const int b = static_cast<int>(bh / p.cache.kv_heads), h = static_cast<int>(bh % p.cache.kv_heads), t = row / p.group;
+  __nv_bfloat16* dst = p.out + b * p.out_member + t * p.out_row + (h * p.group + (row - t * p.group)) * kKv4D + 4 * lane;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(Pairs16<__nv_bfloat16>::pack_pair(x.x * inv, x.y * inv),
+                                              Pairs16<__nv_bfloat16>::pack_pair(x.z * inv, x.w * inv));
+}
+
+// ---------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------
 struct APlan {
@@ -584,21 +1198,36 @@ static int build_attn(const ps_kv4_attn_args* a, APlan* plan, bool host_only) {
   const int64_t rows = static_cast<int64_t>(a->q_tokens) * p.group;
   if (rows > (1 << 30)) return fail(PS_ERR_UNSUPPORTED, "%lld query rows of a K/V head", (long long)rows);
   p.rows = static_cast<int32_t>(rows);
-  plan->kernel = PS_KV4_ROWS;
-  plan->block_rows = rows <= 8 ? 8 : 16;
+  // The rows kernel reads the cache once per 16 query rows, the tiles kernel once per 256 but takes a
+  // whole 128-row tile's time for them.
+  plan->kernel = a->kernel != PS_KV4_AUTO ? a->kernel : (rows > 32 ? PS_KV4_TILES : PS_KV4_ROWS);
+  const bool tiles_kernel = plan->kernel == PS_KV4_TILES;
+  plan->block_rows = tiles_kernel ? kUnitRows : (rows <= 8 ? 8 : 16);
   p.row_blocks = (p.rows + plan->block_rows - 1) / plan->block_rows;
   p.units = a->cache.members * hk * p.row_blocks;
   const int tiles = (a->kv_tokens + kTileKeys - 1) / kTileKeys;
   const int sms = host_only ? 148 : sm_count();
-  int chunks = a->key_chunks > 0 ? a->key_chunks : choose_chunks(p.units, tiles, 3ll * sms);
-  if (chunks > tiles) chunks = tiles > 0 ? tiles : 1;
-  p.chunks = chunks;
   const double scale = a->scale > 0.f ? a->scale : 1.0 / sqrt(static_cast<double>(kKv4D));
   p.scale_log2 = static_cast<float>(scale * a->cache.k_scale * 1.4426950408889634);
-  if (p.units > (1 << 28) || p.units * p.chunks > 0x7fffffffLL)
-    return fail(PS_ERR_UNSUPPORTED, "grid of %lld CTAs", (long long)(p.units * p.chunks));
-  const int64_t slots = p.units * p.chunks * plan->block_rows;
-  plan->ws_bytes = p.chunks > 1 ? slots * (kKv4D * 4 + 8) : 0;
+  if (p.units > (1 << 26)) return fail(PS_ERR_UNSUPPORTED, "%lld units of work", (long long)p.units);
+  int64_t slots;
+  if (tiles_kernel) {
+    p.chunks = 1;
+    p.min_steps = 2;
+    p.grid = sms;
+    // With fixed lengths the number of steps is known: no CTA without work.
+    const int64_t most = p.units * (tiles > 0 ? tiles : 1);
+    if ((most + p.min_steps - 1) / p.min_steps < p.grid) p.grid = static_cast<int32_t>((most + p.min_steps - 1) / p.min_steps);
+    slots = 2ll * p.grid * kUnitRows;
+    plan->ws_bytes = slots * (kKv4D * 4 + 8) + p.units * static_cast<int64_t>(sizeof(int4));
+  } else {
+    int chunks = a->key_chunks > 0 ? a->key_chunks : choose_chunks(p.units, tiles, 3ll * sms);
+    if (chunks > tiles) chunks = tiles > 0 ? tiles : 1;
+    p.chunks = chunks;
+    slots = p.units * p.chunks * plan->block_rows;
+    plan->ws_bytes = p.chunks > 1 ? slots * (kKv4D * 4 + 8) : 0;
+  }
+  if (p.units * p.chunks > 0x7fffffffLL) return fail(PS_ERR_UNSUPPORTED, "grid of %lld CTAs", (long long)(p.units * p.chunks));
   if (!host_only && plan->ws_bytes > 0) {
     if (!a->workspace || a->workspace_bytes < plan->ws_bytes)
       return fail(PS_ERR_NULL, "workspace of %lld bytes needed (ps_kv4_attention_workspace), %lld given",
@@ -607,6 +1236,7 @@ static int build_attn(const ps_kv4_attn_args* a, APlan* plan, bool host_only) {
   }
   p.ws_o = static_cast<float*>(a->workspace);
   p.ws_ml = reinterpret_cast<float2*>(static_cast<unsigned char*>(a->workspace) + slots * kKv4D * 4);
+  p.ws_units = reinterpret_cast<int4*>(p.ws_ml + slots);
   return PS_OK;
 }
 
@@ -631,7 +1261,8 @@ static cudaError_t allow_smem(const void* fn, int bytes) {
 }
 
 template <typename... A>
-static cudaError_t launch(void (*fn)(A...), int64_t blocks, int threads, int smem, cudaStream_t stream, A... args) {
+static cudaError_t launch(void (*fn)(A...), int64_t blocks, int threads, int smem, cudaStream_t stream,
+                          std::common_type_t<A>... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(threads);
@@ -670,6 +1301,15 @@ extern "C" int32_t ps_attention_kv4(const ps_kv4_attn_args* args, void* stream) 
   if (rc != PS_OK || plan.params.units == 0) return rc;
   const ps::AParams& p = plan.params;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (plan.kernel == PS_KV4_TILES) {
+    cudaError_t err = ps::allow_smem(reinterpret_cast<const void*>(ps::kv4_tiles_kernel), ps::kTilesSmem);
+    if (err == cudaSuccess)
+      err = ps::launch(ps::kv4_tiles_kernel, p.grid, ps::kTilesThreads, ps::kTilesSmem, s, p, args->cache.members);
+    if (err == cudaSuccess)
+      err = ps::launch(ps::kv4_merge_kernel, p.units * (ps::kUnitRows / 8), 256, 0, s, p);
+    if (err != cudaSuccess) return ps::fail(PS_ERR_LAUNCH, "kv4 attention launch: %s", cudaGetErrorString(err));
+    return PS_OK;
+  }
   const int smem = static_cast<int>(sizeof(ps::RowsShared)) + 128;
   auto fn = plan.block_rows == 8 ? ps::kv4_rows_kernel<1> : ps::kv4_rows_kernel<2>;
   cudaError_t err = ps::allow_smem(reinterpret_cast<const void*>(fn), smem);

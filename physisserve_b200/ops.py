@@ -972,19 +972,21 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, kv_
     if code is None:
         raise PrepError(f"kernel {kernel!r} is not one of {sorted(_KV4_KERNELS)}")
     rows, lens = table.shape[1] * page_rows, 0
+    # (kv_tokens keeps its name: a lengths tensor that the caller made for this call alone must live until
+    # the launch, or `out` could be allocated in its memory.)
     if kv_tokens is None:
-        kv_tokens = rows
+        most = rows
     elif isinstance(kv_tokens, torch.Tensor):
         if kv_tokens.dtype is not torch.int32 or kv_tokens.shape != (members,) or not kv_tokens.is_contiguous():
             raise PrepError(f"kv_tokens must be an int or a contiguous int32 [{members}] tensor")
         if kv_tokens.get_device() != device_index:
             raise PrepError(f"kv_tokens is on {kv_tokens.device}, the cache on {pages.device}")
         lens = kv_tokens.data_ptr()
-        kv_tokens = rows if max_kv_tokens is None else int(max_kv_tokens)
+        most = rows if max_kv_tokens is None else int(max_kv_tokens)
     else:
-        kv_tokens = int(kv_tokens)
-    if not 0 <= kv_tokens <= rows:
-        raise PrepError(f"kv_tokens={kv_tokens} outside the {rows} rows of the page table")
+        most = int(kv_tokens)
+    if not 0 <= most <= rows:
+        raise PrepError(f"kv_tokens={most} outside the {rows} rows of the page table")
     if out is None:
         out = torch.empty(members, Lq, C, device=q.device, dtype=torch.bfloat16)
     elif out.dtype is not torch.bfloat16 or out.get_device() != device_index or out.shape[:2] != q.shape[:2]:
@@ -993,7 +995,7 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, kv_
     if Lq == 0:
         return out
     args = ctypes.create_string_buffer(_ATTN4.size)
-    _ATTN4.pack_into(args, 0, heads, Lq, kv_tokens, causal_block, scale or 0.0, code, key_chunks, 0, q.data_ptr(), *qs,
+    _ATTN4.pack_into(args, 0, heads, Lq, most, causal_block, scale or 0.0, code, key_chunks, 0, q.data_ptr(), *qs,
                      out.data_ptr(), *os_, lens, 0, 0, *cache)
     lib = _lib.load()
     with _on_device(device_index):

@@ -336,7 +336,7 @@ ATTENDS = [
 ]
 
 
-@pytest.mark.parametrize("kernel", ["auto", "rows"])
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
 @pytest.mark.parametrize("chunks", [0, 1, 3])
 @pytest.mark.parametrize("case", ATTENDS)
 def test_attention_matches_64_bits(case, chunks, kernel):
@@ -351,7 +351,7 @@ def test_attention_matches_64_bits(case, chunks, kernel):
     assert ops.kv4_counters() == (0, 0, 0)
 
 
-@pytest.mark.parametrize("kernel", ["auto", "rows"])
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
 @pytest.mark.parametrize("Lq,cb,chunks", [(1, 0, 0), (3, 1, 4), (200, 0, 2), (200, 60, 0)])
 def test_attention_ragged_lengths(Lq, cb, chunks, kernel):
     """Lengths on the device: zero, one, inside a page, inside a tile, the whole table, beyond it (clamped)."""
@@ -367,7 +367,7 @@ def test_attention_ragged_lengths(Lq, cb, chunks, kernel):
     check_attention(short, q, k, v, [min(max(n, 0), 300) for n in lens], 4, cb)
 
 
-@pytest.mark.parametrize("kernel", ["auto", "rows"])
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
 @pytest.mark.parametrize("Lq", [1, 200])
 def test_attention_never_reads_behind_the_window(Lq, kernel):
     """Table entries behind the window name no page, unwritten rows hold 0xff: neither shows, none is counted."""
@@ -382,7 +382,7 @@ def test_attention_never_reads_behind_the_window(Lq, kernel):
     assert ops.kv4_counters() == (0, 0, 0)
 
 
-@pytest.mark.parametrize("kernel", ["auto", "rows"])
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
 @pytest.mark.parametrize("Lq,page_rows", [(1, 16), (2, 128), (150, 32), (150, 128)])
 def test_attention_leaves_bad_pages_out(Lq, page_rows, kernel):
     rows = 500
@@ -402,7 +402,7 @@ def test_attention_leaves_bad_pages_out(Lq, page_rows, kernel):
     ops.kv4_counters()
 
 
-@pytest.mark.parametrize("kernel", ["auto", "rows"])
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
 @pytest.mark.parametrize("Lq", [1, 300])
 def test_attention_scores_that_grow_along_the_window(Lq, kernel):
     """The running reference has to move many times, by far more than 2^8."""
@@ -418,7 +418,7 @@ def test_attention_scores_that_grow_along_the_window(Lq, kernel):
         check_attention(got, q, k, v, [rows], 2)
 
 
-@pytest.mark.parametrize("kernel", ["auto", "rows"])
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
 @pytest.mark.parametrize("Lq", [2, 140])
 @pytest.mark.parametrize("size", [2.0 ** -100, 2.0 ** -14, 1e4, 2.0 ** 80, 0.0])
 def test_attention_query_rows_of_any_size(size, Lq, kernel):
@@ -430,7 +430,7 @@ def test_attention_query_rows_of_any_size(size, Lq, kernel):
     check_attention(got, q, k, v, [200], 2, scale=scale)
 
 
-@pytest.mark.parametrize("kernel", ["auto", "rows"])
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
 @pytest.mark.parametrize("Lq", [3, 140])
 def test_attention_non_finite_queries_stay_in_their_rows(Lq, kernel):
     pages, table, k, v = fill(1, 300, 2, 128, 12)
@@ -444,7 +444,7 @@ def test_attention_non_finite_queries_stay_in_their_rows(Lq, kernel):
     assert torch.equal(got, clean)
 
 
-@pytest.mark.parametrize("kernel", ["auto", "rows"])
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
 @pytest.mark.parametrize("Lq", [2, 150])
 def test_attention_strides_and_outputs_in_place(Lq, kernel):
     """Q as [B, L, H, D] out of a wider buffer, the output into a wider one; nothing beside it is written."""
