@@ -124,6 +124,36 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
       : "memory");
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 f2_add(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// Waits for the tensor-memory loads issued so far, one of which filled r: nothing that reads r can be
+// moved ahead of the wait.
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                 "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                 "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
+                 "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
+}
+// 16 consecutive fp32 columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
 struct RowsShared {
   alignas(128) unsigned char stage[kStages][kTileBytes];
   alignas(8) unsigned long long full[kStages], empty[kStages];
@@ -519,32 +549,40 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const __grid_constant_
 // sum) in two workspace slots per CTA; kv4_merge_kernel joins them.
 //
 // CTA of four warpgroups:
-//   warps 0-3    dequantise: each thread reads 16 bytes (32 elements) of four keys of K, then of V, one
-//                tile ahead in registers, and writes them as fp16 into the 128-byte swizzled tiles that the
-//                tensor core reads.  The packed bytes come from L2 or HBM straight into registers: a
-//                tile of K and V is 18 KB where it would be 64 KB in bf16;
+//   warp 14      brings the packed K and V of the tiles (9 KB each) into a ring of three shared-memory slots,
+//                one bulk copy per page;
+//   warps 0-3    dequantise: fp16 tiles in the 128-byte swizzled layout that the tensor core reads, two of K
+//                and two of V;
 //   warps 4-7    softmax of query tile 0, warps 8-11 of tile 1: a query row per thread (TMEM lane = row);
-//                they also bring the row's Q, scaled to fp16, into shared memory;
-//   warp 12      owns the tensor memory (512 columns: O0 | S0 | O1 | S1) and issues the MMAs in the order
-//                PV0(t), S0(t+1), PV1(t), S1(t+1), so that one tile's products run under the other's
-//                exponentials.  P overwrites the S columns that were read; P V starts on the first half of
-//                the keys while the second half is exponentiated.
+//                they also bring the row's Q, scaled to fp16, into shared memory.  The two warps of an SM
+//                sub-partition take turns at exponentiating: side by side they would wait for the products
+//                side by side too, and the special-function unit and the tensor core would idle in turn
+//                instead of overlapping;
+//   warps 12, 13 one thread each issues the MMAs of query tile 0 / 1, in the order PV(t), S(t+1): two
+//                issuers, so that neither tile's products wait behind the other's softmax, and the time
+//                between two issues of one (descriptors, barrier tests) is filled by the other's.  P
+//                overwrites the S columns that were read; P V starts on the first half of the keys while
+//                the second half is exponentiated.  Warp 12 owns the tensor memory (512 columns:
+//                O0 | S0 | O1 | S1).
 // tcgen05.mma operations of one thread complete in issue order, so a commit after S_i(t+1) also reports
 // P_i(t) V(t) done.  All waits are bounded: one that runs out raises the CTA's abort flag, every role
-// leaves its loop, the MMA warp waits for its MMAs and frees the tensor memory.
+// leaves its loop, the issuers wait for their MMAs and the tensor memory is freed.
 constexpr int kM = 128;
 constexpr int kUnitRows = 2 * kM;
 constexpr int kTile16 = kM * kKv4D * 2;    // bytes of a 128 x 128 fp16 tile
 constexpr int kHalf16 = kTile16 / 2;       // its 64-column half
+constexpr int kRawBytes = kTileKeys * kKv4Row;  // a packed tile of K or V
+constexpr int kRawSlots = 3;
 constexpr int kTilesThreads = 512;
-constexpr int kDequantRegs = 96, kSoftmaxRegs = 184, kMmaRegs = 48;
-static_assert(kDequantRegs + 2 * kSoftmaxRegs + kMmaRegs <= 512, "register split exceeds the launch's 128 a thread");
-constexpr int kOffQ = 0, kOffK = kOffQ + 2 * kTile16, kOffV = kOffK + 2 * kTile16, kOffBars = kOffV + 2 * kTile16;
+constexpr int kOffQ = 0, kOffK = kOffQ + 2 * kTile16, kOffV = kOffK + 2 * kTile16, kOffRaw = kOffV + 2 * kTile16;
+constexpr int kOffBars = kOffRaw + kRawSlots * kRawBytes;
 enum TBar {
   kQFull, kKFull = kQFull + 2, kKEmpty = kKFull + 2, kVFull = kKEmpty + 2, kVEmpty = kVFull + 2, kSFull = kVEmpty + 2,
-  kPHalf = kSFull + 2, kPFull = kPHalf + 2, kOFinal = kPFull + 2, kMmaDone = kOFinal + 2, kTBars
+  kPHalf = kSFull + 2, kPFull = kPHalf + 2, kOFinal = kPFull + 2, kRawFull = kOFinal + 2, kRawEmpty = kRawFull + kRawSlots,
+  kTurn = kRawEmpty + kRawSlots, kMmaDone = kTurn + 8, kTBars
 };
-constexpr int kOffTmem = kOffBars + 8 * kTBars, kOffAbort = kOffTmem + 4, kOffStart = kOffAbort + 4;
+constexpr int kOffTmem = kOffBars + 8 * kTBars, kOffAbort = kOffTmem + 4, kOffThere = kOffAbort + 4;
+constexpr int kOffStart = (kOffThere + 4 * kRawSlots + 15) & ~15;
 constexpr int kTilesSmem = kOffStart + 32 + 1024;
 static_assert(kTilesSmem <= 227 * 1024, "tiles exceed shared memory");
 __host__ __device__ constexpr int col_o(int i) { return 256 * i; }
@@ -554,15 +592,41 @@ __host__ __device__ constexpr uint32_t idesc16(uint32_t b_mn) {
   return (1u << 4) | (b_mn << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
 }
 
-template <int N> __device__ __forceinline__ void regs_dec() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+// One K = 16 step of S = Q K^T: both operands OFFSET bytes into their tiles.  The descriptor's address
+// field holds address >> 4 and shared addresses stay below 2^18, so the sum cannot carry out of it.
+// Everything is formed inside the statement: descriptors of all steps kept in registers do not fit the
+// issuing warp's share, and a spilled one costs more than the tensor core has queued.
+template <int OFFSET>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t high, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b32 a, b;\n\t.reg .b64 x, y;\n\t"
+      "add.u32 a, %1, %6;\n\tadd.u32 b, %2, %6;\n\t"
+      "mov.b64 x, {a, %3};\n\tmov.b64 y, {b, %3};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %5, p;\n\t}" ::"r"(d),
+      "r"(a_low), "r"(b_low), "r"(high), "r"(acc ? 1u : 0u), "n"(idesc16(0)), "n"(OFFSET >> 4)
+      : "memory");
 }
-template <int N> __device__ __forceinline__ void regs_inc() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+// Step STEP (16 keys) of O += P V: P from tensor memory (8 columns a step), V's key rows 2 KB a step.
+template <int STEP>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_low, uint32_t high, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b32 a, b;\n\t.reg .b64 y;\n\t"
+      "add.u32 a, %1, %6;\n\tadd.u32 b, %2, %7;\n\t"
+      "mov.b64 y, {b, %3};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], y, %5, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_low), "r"(high), "r"(acc ? 1u : 0u), "n"(idesc16(1)), "n"(STEP * 8), "n"(STEP * 128)
+      : "memory");
 }
-// wait_bar inline: the register splits above do not survive a call.
+
+// wait_bar inline (a call costs its registers).  Nearly every wait ends within a few suspended tries; only
+// then is the clock read (it is slow).
 __device__ __forceinline__ bool spin_bar(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   if (bar_test(bar, parity)) return true;
+#pragma unroll 1
+  for (int i = 0; i < 64; ++i)
+    if (bar_try(bar, parity)) return true;
   const unsigned long long start = now_ns();
   for (;;) {
 #pragma unroll 1
@@ -588,33 +652,31 @@ __device__ __forceinline__ int unit_steps(const AParams& p, int n, int qb, int& 
   return max(1, (lim_top + kTileKeys - 1) / kTileKeys);
 }
 
-// A CTA's way through its range of steps; every role walks the same way.
+// A CTA's way through its range of `count` steps; every role walks the same way.
 struct Walk {
-  int b, h, qb, n, lim_top;
+  int b, h, qb, lim_top;
   int j0, j1;        // key tiles of the present segment
   int steps;         // steps of the present unit
-  int64_t at, end;   // step of j0, end of the CTA's range
-  bool first;        // the CTA's first segment
+  int done, count;   // steps before the present segment, steps of the CTA
 
-  __device__ __forceinline__ bool begin(const AParams& p, const int4& start, int64_t s0, int64_t s1) {
+  __device__ __forceinline__ bool begin(const AParams& p, const int4& start, int n_steps) {
     b = start.x;
     h = start.y;
     qb = start.z;
     j0 = start.w;
-    at = s0;
-    end = s1;
-    first = true;
-    return at < end && (open(p), true);
+    done = 0;
+    count = n_steps;
+    if (count == 0) return false;
+    open(p);
+    return true;
   }
   __device__ __forceinline__ void open(const AParams& p) {
-    n = member_len(p, b);
-    steps = unit_steps(p, n, qb, lim_top);
-    j1 = static_cast<int>(min(static_cast<int64_t>(steps), j0 + (end - at)));
+    steps = unit_steps(p, member_len(p, b), qb, lim_top);
+    j1 = min(steps, j0 + (count - done));
   }
   __device__ __forceinline__ bool next(const AParams& p) {
-    at += j1 - j0;
-    if (at >= end) return false;
-    first = false;
+    done += j1 - j0;
+    if (done >= count) return false;
     j0 = 0;
     if (++qb == p.row_blocks) {
       qb = 0;
@@ -626,6 +688,7 @@ struct Walk {
     open(p);
     return true;
   }
+  __device__ __forceinline__ bool first() const { return done == 0; }  // the CTA's first segment
   __device__ __forceinline__ bool two(const AParams& p) const { return qb * kUnitRows + kM < p.rows; }
   __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == steps; }
   __device__ __forceinline__ int64_t unit(const AParams& p) const {
@@ -704,17 +767,22 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      bar_init(bar(kQFull + i), 128);
+      bar_init(bar(kQFull + i), 4);
       bar_init(bar(kKFull + i), 4);
-      bar_init(bar(kKEmpty + i), 1);
+      bar_init(bar(kKEmpty + i), 2);   // both issuers
       bar_init(bar(kVFull + i), 4);
-      bar_init(bar(kVEmpty + i), 1);
+      bar_init(bar(kVEmpty + i), 2);
       bar_init(bar(kSFull + i), 1);
-      bar_init(bar(kPHalf + i), 128);
-      bar_init(bar(kPFull + i), 128);
+      bar_init(bar(kPHalf + i), 4);
+      bar_init(bar(kPFull + i), 4);
       bar_init(bar(kOFinal + i), 1);
     }
-    bar_init(bar(kMmaDone), 1);
+    for (int i = 0; i < kRawSlots; ++i) {
+      bar_init(bar(kRawFull + i), 1);
+      bar_init(bar(kRawEmpty + i), 4);
+    }
+    for (int i = 0; i < 8; ++i) bar_init(bar(kTurn + i), 1);
+    bar_init(bar(kMmaDone), 2);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -740,159 +808,185 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
   const uint32_t tmem = *tmem_slot;
   const int64_t per = range[0];
   const int4 start = *reinterpret_cast<int4*>(range + 2);
-  const int64_t s0 = min(per * blockIdx.x, range[1]), s1 = min(s0 + per, range[1]);
+  const int n_steps = static_cast<int>(max(min(per, range[1] - per * blockIdx.x), int64_t(0)));
   const int shift = p.cache.shift;
   Walk w;
 
   if (warp < 4) {
     // ------------------------------- dequantisers -------------------------------
-    regs_dec<kDequantRegs>();
-    // Lane (r, c): 16-byte chunk c (elements 32c .. 32c+31) of keys 32 i + 8 warp + r, i = 0..3.  A warp
-    // reads 512 contiguous bytes of 8 keys at a time (their page is one: pages hold 16 rows or more).
-    // Chunks 0 and 1 go to the tile's left half, 2 and 3 to its right one, whose rows fall into the same
-    // banks: lanes of the right half write their four 16-byte parts in the order 2 3 0 1, so that
-    // eight lanes of a store cover all banks.
+    // Lane (r, c): 16-byte chunk c (elements 32c .. 32c+31) of keys 32 i + 8 warp + r, i = 0..3.  Chunks 0
+    // and 1 go to the fp16 tile's left half, 2 and 3 to its right one, whose rows fall into the same
+    // banks: lanes of the right half take their four 8-element parts in the order 2 3 0 1, so that eight
+    // lanes of a store cover all banks.
     const int r = lane >> 2, c = lane & 3;
     const bool right = c >= 2;
-    const int half = static_cast<int>(p.cache.head_bytes >> 1);
     const int page_rows = 1 << shift;
-    uint32_t dst[4];  // byte offset of part i (in write order) of key row 8 warp + r
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int part = (c & 1) * 4 + (right ? i ^ 2 : i);
-      dst[i] = (c >> 1) * kHalf16 + (8 * warp + r) * 128 + ((part ^ r) * 16);
-    }
-    uint4 kw[4], vw[4];
-    uint32_t ks[4], vs[4];
-    int64_t page[4];
-    // Pages of the four keys of tile j; -1 where nothing is to be read.
-    auto pages = [&](int j, bool count) {
-#pragma unroll
+    // Byte offset of part 0 (in write order) of key row 8 warp + r; part i is at dst0 ^ (16 i).
+    const uint32_t dst0 = (c >> 1) * kHalf16 + (8 * warp + r) * 128 + ((((c & 1) * 4) ^ (right ? 2 : 0) ^ r) * 16);
+    const uint32_t sel_a = right ? 0x3232 : 0x1010, sel_b = right ? 0x1010 : 0x3232;
+    // One packed tile (slot of ring position u) to the fp16 tile at `tile`, once `empty` has its phase.
+    // `seen`: keys of the tile that any row sees (V only: what a missing or unseen key holds must not
+    // reach the products even times a probability of 0, so its scale becomes 0).
+    auto expand = [&](int u, uint32_t tile, int empty, uint32_t parity, bool wait_empty, int seen) -> bool {
+      const int slot = u % kRawSlots;
+      if (!warp_spin(bar(kRawFull + slot), (u / kRawSlots) & 1, abort_flag)) return false;
+      if (wait_empty && !warp_spin(bar(empty), parity, abort_flag)) return false;
+      const uint32_t raw = sbase + kOffRaw + slot * kRawBytes;
+      const uint32_t there = *reinterpret_cast<volatile uint32_t*>(smem + kOffThere + 4 * slot);
+      const bool all = seen >= kTileKeys && there == (1u << (kTileKeys >> shift)) - 1;
+#pragma unroll 1
       for (int i = 0; i < 4; ++i) {
-        const int key = j * kTileKeys + 32 * i + 8 * warp + r;
-        page[i] = -1;
-        if (key < w.lim_top) {
-          const int32_t x = p.cache.table[w.b * p.cache.table_pages + (key >> shift)];
-          if (static_cast<uint32_t>(x) < p.cache.num_pages) page[i] = x;
-          else if (count && c == 0 && (key & (page_rows - 1)) == 0) atomicAdd(&g_kv4_counts[kKv4BadPages], 1u);
-        }
-      }
-    };
-    auto load = [&](uint4* x, uint32_t* s, int off) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = make_uint4(0, 0, 0, 0);
-        s[i] = 0;
-        if (page[i] >= 0) {
-          const int in_page = (32 * i + 8 * warp + r) & (page_rows - 1);
-          const unsigned char* base = kv4_head(p.cache, page[i], w.h) + off;
-          x[i] = *reinterpret_cast<const uint4*>(base + in_page * 64 + c * 16);
-          s[i] = *reinterpret_cast<const uint16_t*>(base + page_rows * 64 + in_page * 8 + c * 2);
-        }
-      }
-    };
-    auto expand = [&](const uint4* x, const uint32_t* s, uint32_t tile) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t s2 = kv4_scales(s[i]);
-        const uint32_t sa = __byte_perm(s2, s2, right ? 0x3232 : 0x1010), sb = __byte_perm(s2, s2, right ? 0x1010 : 0x3232);
-        const uint32_t q[4] = {right ? x[i].z : x[i].x, right ? x[i].w : x[i].y, right ? x[i].x : x[i].z,
-                               right ? x[i].y : x[i].w};
+        const int key = 32 * i + 8 * warp + r, in_page = key & (page_rows - 1);
+        const uint32_t seg = raw + (key >> shift) * (page_rows * kKv4Row);
+        const uint32_t src = seg + in_page * 64 + c * 16 + (right ? 8 : 0);
+        uint32_t x[4];
+        asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(x[0]), "=r"(x[1]) : "r"(src));
+        asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(x[2]), "=r"(x[3]) : "r"(src ^ 8));
+        uint16_t two;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(two) : "r"(seg + page_rows * 64 + in_page * 8 + c * 2));
+        uint32_t s2 = two;
+        if (!all && (key >= seen || !((there >> (key >> shift)) & 1))) s2 = 0;
+        const uint32_t sc = kv4_scales(s2);
+        const uint32_t sa = __byte_perm(sc, sc, sel_a), sb = __byte_perm(sc, sc, sel_b);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           uint32_t o[4];
-          kv4_unpack(q[k], o);
-          const uint32_t sc = k < 2 ? sa : sb;
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(tile + 32 * i * 128 + dst[k]), "r"(h2_mul(o[0], sc)),
-                       "r"(h2_mul(o[1], sc)), "r"(h2_mul(o[2], sc)), "r"(h2_mul(o[3], sc))
+          kv4_unpack(x[k], o);
+          const uint32_t f = k < 2 ? sa : sb;
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(tile + 32 * i * 128 + (dst0 ^ (16 * k))),
+                       "r"(h2_mul(o[0], f)), "r"(h2_mul(o[1], f)), "r"(h2_mul(o[2], f)), "r"(h2_mul(o[3], f))
                        : "memory");
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
+      if (lane == 0) bar_arrive(bar(kRawEmpty + slot));
+      return true;
     };
     int t = 0;
     bool ok = true;
-    for (bool more = w.begin(p, start, s0, s1); ok && more; more = w.next(p)) {
-      pages(w.j0, true);
-      load(kw, ks, 0);
-      load(vw, vs, half);
+    for (bool more = w.begin(p, start, n_steps); ok && more; more = w.next(p)) {
       for (int j = w.j0; j < w.j1; ++j, ++t) {
         const int st = t & 1;
         const uint32_t parity = ((t >> 1) & 1) ^ 1;
-        if (j + 1 < w.j1) pages(j + 1, true);
-        if (t >= 2 && !(ok = warp_spin(bar(kKEmpty + st), parity, abort_flag))) break;
-        expand(kw, ks, sbase + kOffK + st * kTile16);
+        if (!(ok = expand(2 * t, sbase + kOffK + st * kTile16, kKEmpty + st, parity, t >= 2, kTileKeys))) break;
         if (lane == 0) bar_arrive(bar(kKFull + st));
-        if (j + 1 < w.j1) load(kw, ks, 0);
-        if (t >= 2 && !(ok = warp_spin(bar(kVEmpty + st), parity, abort_flag))) break;
-        expand(vw, vs, sbase + kOffV + st * kTile16);
+        if (!(ok = expand(2 * t + 1, sbase + kOffV + st * kTile16, kVEmpty + st, parity, t >= 2,
+                          w.lim_top - j * kTileKeys)))
+          break;
         if (lane == 0) bar_arrive(bar(kVFull + st));
-        if (j + 1 < w.j1) load(vw, vs, half);
       }
     }
   } else if (warp >= 12) {
-    regs_dec<kMmaRegs>();
-    if (warp == 12 && lane == 0) {
-      // ------------------------------- MMA issuer -------------------------------
-      const uint32_t id_s = idesc16(0), id_pv = idesc16(1);
-      const uint64_t qd0 = smem_desc(sbase + kOffQ, 16, 1024), kd0 = smem_desc(sbase + kOffK, 16, 1024);
-      const uint64_t vd0 = smem_desc(sbase + kOffV, kHalf16, 1024);
-      auto issue_s = [&](int i, int t) {
-        const uint64_t qd = qd0 + (i ? kTile16 >> 4 : 0), kd = kd0 + ((t & 1) ? kTile16 >> 4 : 0);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint64_t off = static_cast<uint64_t>(((k >> 2) * kHalf16 + (k & 3) * 32) >> 4);
-          tc_mma(tmem + col_s(i), qd + off, kd + off, id_s, k > 0);
-        }
-      };
-      // Four 16-key steps of P V from step k0.
-      auto issue_pv = [&](int i, int t, int k0, bool fresh) {
-        const uint64_t vd = vd0 + ((t & 1) ? kTile16 >> 4 : 0);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          tc_mma_ts(tmem + col_o(i), tmem + col_s(i) + (k0 + k) * 8, vd + static_cast<uint64_t>((k0 + k) * 128), id_pv,
-                    !(fresh && k0 + k == 0));
-      };
-      int t = 0, tq[2] = {0, 0}, segs[2] = {0, 0};  // key tiles; tiles and segments of each query tile
+    if (warp == 14) {
+      // ------------------------------- bulk copies -------------------------------
+      const uint32_t bytes = static_cast<uint32_t>(p.cache.head_bytes >> 1);  // K or V of a head in a page
+      const int per_tile = kTileKeys >> shift;
+      int u = 0;
       bool ok = true;
-      for (bool more_segs = w.begin(p, start, s0, s1); ok && more_segs; more_segs = w.next(p)) {
-        const int nq = w.two(p) ? 2 : 1, count = w.j1 - w.j0;
-        if (!(ok = spin_bar(bar(kKFull + (t & 1)), (t >> 1) & 1, abort_flag))) break;
+      for (bool more = w.begin(p, start, n_steps); ok && more; more = w.next(p)) {
+        // Lane i: table entry of the tile's page i, a tile ahead.
+        auto entry_of = [&](int j) {
+          int32_t x = -1;
+          if (lane < per_tile && j < w.j1 && j * kTileKeys + (lane << shift) < w.lim_top)
+            x = p.cache.table[w.b * p.cache.table_pages + ((j * kTileKeys) >> shift) + lane];
+          return x;
+        };
+        int32_t entry = entry_of(w.j0);
+        for (int j = w.j0; ok && j < w.j1; ++j) {
+          const bool wanted = lane < per_tile && j * kTileKeys + (lane << shift) < w.lim_top;
+          const bool valid = wanted && static_cast<uint32_t>(entry) < p.cache.num_pages;
+          if (wanted && !valid) atomicAdd(&g_kv4_counts[kKv4BadPages], 1u);
+          const uint32_t there = __ballot_sync(0xffffffffu, valid);
+          const unsigned char* src = kv4_head(p.cache, valid ? entry : 0, w.h);
+          entry = entry_of(j + 1);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (i >= nq) continue;
-          if (!(ok = spin_bar(bar(kQFull + i), segs[i] & 1, abort_flag))) break;
-          ++segs[i];
-          tc_fence_after();
-          issue_s(i, t);
-          tc_commit(bar(kSFull + i));
+          for (int kv = 0; kv < 2; ++kv, ++u) {
+            const int slot = u % kRawSlots;
+            if (u >= kRawSlots && !(ok = warp_spin(bar(kRawEmpty + slot), ((u / kRawSlots) & 1) ^ 1, abort_flag))) break;
+            if (lane == 0) {
+              *reinterpret_cast<volatile uint32_t*>(smem + kOffThere + 4 * slot) = there;
+              bar_expect_tx(bar(kRawFull + slot), __popc(there) * bytes);
+            }
+            __syncwarp();
+            if (valid)
+              bulk_load(sbase + kOffRaw + slot * kRawBytes + lane * bytes, src + kv * bytes, bytes, bar(kRawFull + slot));
+          }
         }
-        if (!ok) break;
+      }
+      // Every copy has landed before the CTA may exit.
+      volatile int never = 0;
+      for (int x = u > kRawSlots ? u - kRawSlots : 0; x < u; ++x)
+        spin_bar(bar(kRawFull + x % kRawSlots), (x / kRawSlots) & 1, &never);
+      __syncwarp();
+    } else if (warp < 14 && lane == 0) {
+      // ------------------------------- MMA issuers -------------------------------
+      const int i = warp - 12;
+      // Low words of the descriptors (address and leading byte offset); the high word is the same for all.
+      const uint64_t q_desc = smem_desc(sbase + kOffQ + i * kTile16, 16, 1024);
+      const uint32_t high = static_cast<uint32_t>(q_desc >> 32), q_low = static_cast<uint32_t>(q_desc);
+      const uint32_t k_low = static_cast<uint32_t>(smem_desc(sbase + kOffK, 16, 1024));
+      const uint32_t v_low = static_cast<uint32_t>(smem_desc(sbase + kOffV, kHalf16, 1024));
+      const uint32_t s_col = tmem + col_s(i), o_col = tmem + col_o(i);
+      auto issue_s = [&](int t) {
+        const uint32_t k = k_low + ((t & 1) ? kTile16 >> 4 : 0);
+        mma_ss<0>(s_col, q_low, k, high, false);
+        mma_ss<32>(s_col, q_low, k, high, true);
+        mma_ss<64>(s_col, q_low, k, high, true);
+        mma_ss<96>(s_col, q_low, k, high, true);
+        mma_ss<kHalf16>(s_col, q_low, k, high, true);
+        mma_ss<kHalf16 + 32>(s_col, q_low, k, high, true);
+        mma_ss<kHalf16 + 64>(s_col, q_low, k, high, true);
+        mma_ss<kHalf16 + 96>(s_col, q_low, k, high, true);
+      };
+      // Four 16-key steps of P V: the first or the second half of the tile's keys.
+      auto issue_pv = [&](int t, bool second, bool fresh) {
+        const uint32_t v = v_low + ((t & 1) ? kTile16 >> 4 : 0) + (second ? 4 * 128 : 0);
+        const uint32_t a = s_col + (second ? 32 : 0);
+        mma_ts<0>(o_col, a, v, high, !fresh);
+        mma_ts<1>(o_col, a, v, high, true);
+        mma_ts<2>(o_col, a, v, high, true);
+        mma_ts<3>(o_col, a, v, high, true);
+      };
+      int t = 0, tq = 0, segs = 0;  // key tiles; tiles and segments of this query tile
+      bool ok = true;
+      for (bool more_segs = w.begin(p, start, n_steps); ok && more_segs; more_segs = w.next(p)) {
+        const int count = w.j1 - w.j0;
+        if (i == 1 && !w.two(p)) {
+          // No rows here: only report the tiles as read once they are there.
+          for (int jj = 0; ok && jj < count; ++jj, ++t) {
+            if (!(ok = spin_bar(bar(kKFull + (t & 1)), (t >> 1) & 1, abort_flag))) break;
+            bar_arrive(bar(kKEmpty + (t & 1)));
+            if (!(ok = spin_bar(bar(kVFull + (t & 1)), (t >> 1) & 1, abort_flag))) break;
+            bar_arrive(bar(kVEmpty + (t & 1)));
+          }
+          continue;
+        }
+        if (!(ok = spin_bar(bar(kKFull + (t & 1)), (t >> 1) & 1, abort_flag))) break;
+        if (!(ok = spin_bar(bar(kQFull + i), segs & 1, abort_flag))) break;
+        ++segs;
+        tc_fence_after();
+        issue_s(t);
+        tc_commit(bar(kSFull + i));
         tc_commit(bar(kKEmpty + (t & 1)));
-        for (int jj = 0; ok && jj < count; ++jj, ++t) {
+        for (int jj = 0; jj < count; ++jj, ++t, ++tq) {
           const bool more = jj + 1 < count;
           if (!(ok = spin_bar(bar(kVFull + (t & 1)), (t >> 1) & 1, abort_flag))) break;
+          if (!(ok = spin_bar(bar(kPHalf + i), tq & 1, abort_flag))) break;
+          tc_fence_after();
+          issue_pv(t, false, jj == 0);
           if (more && !(ok = spin_bar(bar(kKFull + ((t + 1) & 1)), ((t + 1) >> 1) & 1, abort_flag))) break;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (i >= nq) continue;
-            if (!(ok = spin_bar(bar(kPHalf + i), tq[i] & 1, abort_flag))) break;
-            tc_fence_after();
-            issue_pv(i, t, 0, jj == 0);
-            if (!(ok = spin_bar(bar(kPFull + i), tq[i] & 1, abort_flag))) break;
-            ++tq[i];
-            tc_fence_after();
-            issue_pv(i, t, 4, false);
-            const bool last = i == nq - 1;
-            if (more) {
-              issue_s(i, t + 1);
-              tc_commit(bar(kSFull + i));
-              if (last) tc_commit(bar(kKEmpty + ((t + 1) & 1)));
-            } else {
-              tc_commit(bar(kOFinal + i));
-            }
-            if (last) tc_commit(bar(kVEmpty + (t & 1)));
+          if (!(ok = spin_bar(bar(kPFull + i), tq & 1, abort_flag))) break;
+          tc_fence_after();
+          issue_pv(t, true, false);
+          if (more) {
+            issue_s(t + 1);
+            tc_commit(bar(kSFull + i));
+            tc_commit(bar(kVEmpty + (t & 1)));
+            tc_commit(bar(kKEmpty + ((t + 1) & 1)));
+          } else {
+            tc_commit(bar(kOFinal + i));
+            tc_commit(bar(kVEmpty + (t & 1)));
           }
         }
       }
@@ -901,31 +995,36 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
     __syncwarp();
   } else {
     // ------------------------------- softmax -------------------------------
-    regs_inc<kSoftmaxRegs>();
     const int qi = (warp - 4) >> 2;
     const int row = (warp & 3) * 32 + lane;  // row of the query tile = TMEM lane
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t s_addr = lanes + col_s(qi), o_addr = lanes + col_o(qi);
     const int segs_tile = kTileKeys >> shift;
-    int n_tiles = 0, n_segs = 0;
+    int n_tiles = 0, n_segs = 0, n_turns = 0;
+    const int turn = kTurn + 2 * (warp & 3);  // barrier turn + i: this pair's warp of tile i may go
     bool ok = true;
-    for (bool more = w.begin(p, start, s0, s1); ok && more; more = w.next(p)) {
+    for (bool more = w.begin(p, start, n_steps); ok && more; more = w.next(p)) {
       if (qi == 1 && !w.two(p)) continue;
-      const int q_row = w.qb * kUnitRows + qi * kM + row;  // of the K/V head's rows
-      const int token = min(q_row, p.rows - 1) / p.group;
-      const int lim = token_limit(p, w.n, token);
-      // Rows grow downwards, and so do their limits: the tile's first row sees the fewest keys.
-      const int lim_low = token_limit(p, w.n, min(w.qb * kUnitRows + qi * kM, p.rows - 1) / p.group);
-      const int64_t head_off = static_cast<int64_t>(w.h * p.group + (min(q_row, p.rows - 1) - token * p.group)) * kKv4D;
+      // This thread's query row (rows of the K/V head), its token and its offset in q and out.
+      auto q_row = [&] { return w.qb * kUnitRows + qi * kM + row; };
+      auto row_at = [&](const int64_t member, const int64_t token_stride) {
+        const int r = min(q_row(), p.rows - 1), t = r / p.group;
+        return w.b * member + t * token_stride + (w.h * p.group + (r - t * p.group)) * kKv4D;
+      };
+      const int n = member_len(p, w.b);
+      const int lim = token_limit(p, n, min(q_row(), p.rows - 1) / p.group);
+      // Rows grow downwards and their limits with them: the first tile in which a row of this query tile
+      // does not see every key.
+      const int j_mask = token_limit(p, n, min(w.qb * kUnitRows + qi * kM, p.rows - 1) / p.group) / kTileKeys;
       float scale;
       {
-        // This thread's query row: scaled to fp16 and stored 128-byte swizzled.
+        // Q, scaled to fp16 and stored 128-byte swizzled.
         uint4 x[16];
-        const __nv_bfloat16* src = p.q + w.b * p.q_member + token * p.q_row + head_off;
+        const __nv_bfloat16* src = p.q + row_at(p.q_member, p.q_row);
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          x[i] = q_row < p.rows ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0, 0, 0, 0);
+          x[i] = q_row() < p.rows ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0, 0, 0, 0);
           top = __vmaxu2(top, __vmaxu2(__vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu),
                                        __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu)));
         }
@@ -945,36 +1044,55 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         tc_fence_before();
-        bar_arrive(bar(kQFull + qi));
+        __syncwarp();
+        if (lane == 0) bar_arrive(bar(kQFull + qi));
       }
+      // Does the segment have a page that is not in the pool?  Its keys are left out, tile by tile.
+      auto bad_pages = [&](int first, int end) {  // bit i: page first + 32 k + i, k = 0, 1, .., is not there
+        bool bad = false;
+        for (int i = first + lane; i < end; i += 32)
+          bad |= static_cast<uint32_t>(p.cache.table[w.b * p.cache.table_pages + i]) >= p.cache.num_pages;
+        return __ballot_sync(0xffffffffu, bad);
+      };
+      const int pages_seen = (w.lim_top + (1 << shift) - 1) >> shift;
+      const bool any_bad = bad_pages(w.j0 * segs_tile, min(w.j1 * segs_tile, pages_seen)) != 0;
       float m = -INFINITY, l = 0.f;
       for (int j = w.j0; j < w.j1; ++j, ++n_tiles) {
-        // Pages of the tile that are not in the pool: their keys are left out.
-        int32_t page = 0;
-        if (lane < segs_tile && j * kTileKeys + (lane << shift) < w.lim_top)
-          page = p.cache.table[w.b * p.cache.table_pages + ((j * kTileKeys) >> shift) + lane];
-        const uint32_t bad = __ballot_sync(0xffffffffu, static_cast<uint32_t>(page) >= p.cache.num_pages);
         if (!(ok = warp_spin(bar(kSFull + qi), n_tiles & 1, abort_flag))) break;
         tc_fence_after();
-        uint32_t s[128];
+        // Two passes over the scores in tensor memory, 32 columns at a time with the next 32 on their way:
+        // the row's maximum, then the probabilities.  The loops stay rolled: a sub-partition runs four
+        // roles' code side by side, and unrolled they wait for instructions more than for anything else.
+        const bool masked = j >= j_mask || any_bad;
+        const uint32_t bad = any_bad ? bad_pages(j * segs_tile, min((j + 1) * segs_tile, pages_seen)) : 0;
+        const int valid = lim - j * kTileKeys;
+        auto hide = [&](uint32_t* x, int first) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, s + 32 * c);
-        tmem_wait_ld();
-        if ((j + 1) * kTileKeys > lim_low || bad) {
-          const int valid = lim - j * kTileKeys;
+          for (int i = 0; i < 32; ++i)
+            if (first + i >= valid || ((bad >> ((first + i) >> shift)) & 1)) x[i] = __float_as_uint(-INFINITY);
+        };
+        uint32_t xa[32], xb[32];
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto largest = [&](const uint32_t* y) {
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (i >= valid || ((bad >> (i >> shift)) & 1)) s[i] = __float_as_uint(-INFINITY);
+          for (int i = 0; i < 32; i += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              mx[e] = max3(mx[e], __uint_as_float(y[i + 2 * e]), __uint_as_float(y[i + 2 * e + 1]));
+        };
+        tmem_ld32(s_addr, xa);
+#pragma unroll 1
+        for (int col = 0; col < 128; col += 64) {
+          tmem_wait_ld32(xa);
+          tmem_ld32(s_addr + col + 32, xb);
+          if (masked) hide(xa, col);
+          largest(xa);
+          tmem_wait_ld32(xb);
+          tmem_ld32(s_addr + ((col + 64) & 127), xa);  // the last one is the second pass's first
+          if (masked) hide(xb, col + 32);
+          largest(xb);
         }
-        float mx[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) mx[e] = __uint_as_float(s[e]);
-#pragma unroll
-        for (int i = 8; i < 128; i += 8)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(s[i + e]));
-        const float top =
-            fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))) * scale;
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
         // The reference moves only when a score exceeds it by more than 8: P is exact for any reference.
         const bool grow = top > m + 8.f;
         const float alpha = grow ? fast_exp2(m - top) : 1.f;
@@ -985,45 +1103,65 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
         // O holds this segment's earlier tiles (their P V have completed: S was committed after them).
         if (__any_sync(0xffffffffu, grow) && j > w.j0) {
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t o[32];
-            tmem_ld32(o_addr + 32 * c, o);
+          for (int c = 0; c < 8; ++c) {
+            uint32_t o[16];
+            tmem_ld16(o_addr + 16 * c, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-            tmem_st32(o_addr + 32 * c, o);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st16(o_addr + 16 * c, o);
           }
         }
         const float ref = m == -INFINITY ? 0.f : m;
-        float ls[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
+        const f32x2 scale2 = f2_make(scale, scale), ref2 = f2_make(-ref, -ref);
+        f32x2 sum[2] = {0, 0};
+        // Tile 0's k-th turn follows tile 1's (k-1)-th, tile 1's k-th follows tile 0's k-th.
+        if (w.two(p)) {
+          if (qi + n_turns > 0 && !(ok = warp_spin(bar(turn + qi), (n_turns - 1 + qi) & 1, abort_flag))) break;
+          ++n_turns;
+        }
+        // 32 scores to probabilities, over columns that both passes have read.
+        auto exponentiate = [&](const uint32_t* y, uint32_t p_col) {
           uint32_t pk[16];
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
-            const float x0 = fast_exp2(fmaf(__uint_as_float(s[32 * h + 2 * c]), scale, -ref));
-            const float x1 = fast_exp2(fmaf(__uint_as_float(s[32 * h + 2 * c + 1]), scale, -ref));
-            ls[(c & 1) * 2] += x0;
-            ls[(c & 1) * 2 + 1] += x1;
+            float x0, x1;
+            f2_split(f2_fma(f2_make(__uint_as_float(y[2 * c]), __uint_as_float(y[2 * c + 1])), scale2, ref2), x0, x1);
+            x0 = fast_exp2(x0);
+            x1 = fast_exp2(x1);
+            sum[c & 1] = f2_add(sum[c & 1], f2_make(x0, x1));
             pk[c] = h2_pack(x0, x1);
           }
-          tmem_st16(s_addr + 16 * h, pk);
-          if (h & 1) {
-            tmem_wait_st();
-            tc_fence_before();
-            bar_arrive(bar((h == 1 ? kPHalf : kPFull) + qi));
-          }
+          tmem_st16(s_addr + p_col, pk);
+        };
+#pragma unroll 1
+        for (int col = 0; col < 128; col += 64) {
+          tmem_wait_ld32(xa);
+          tmem_ld32(s_addr + col + 32, xb);
+          if (masked) hide(xa, col);
+          exponentiate(xa, col >> 1);
+          tmem_wait_ld32(xb);
+          if (col == 0) tmem_ld32(s_addr + 64, xa);
+          if (masked) hide(xb, col + 32);
+          exponentiate(xb, (col >> 1) + 16);
+          if (col != 0 && w.two(p) && lane == 0) bar_arrive(bar(turn + 1 - qi));
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(bar((col == 0 ? kPHalf : kPFull) + qi));
         }
-        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+        float l0, l1;
+        f2_split(f2_add(sum[0], sum[1]), l0, l1);
+        l += l0 + l1;
       }
       if (!ok) break;
       if (!(ok = warp_spin(bar(kOFinal + qi), n_segs & 1, abort_flag))) break;
       ++n_segs;
       tc_fence_after();
-      const bool live = q_row < p.rows;
+      const bool live = q_row() < p.rows;
       if (w.whole()) {
         const float inv = l == 0.f ? 0.f : p.cache.v_scale / l;
-        __nv_bfloat16* dst = p.out + w.b * p.out_member + token * p.out_row + head_off;
+        __nv_bfloat16* dst = p.out + row_at(p.out_member, p.out_row);
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t o[32];
@@ -1043,7 +1181,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
           }
         }
       } else {
-        const int64_t slot = (2ll * blockIdx.x + (w.first ? 0 : 1)) * kUnitRows + qi * kM + row;
+        const int64_t slot = (2ll * blockIdx.x + (w.first() ? 0 : 1)) * kUnitRows + qi * kM + row;
         float* dst = p.ws_o + slot * kKv4D;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
@@ -1060,8 +1198,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
         p.ws_ml[slot] = make_float2(m, l);
       }
       if (qi == 0 && row == 0 && w.j0 == 0) {
-        const int last = static_cast<int>((w.at + w.steps - 1) / per);
-        p.ws_units[w.unit(p)] = make_int4(static_cast<int>(blockIdx.x), last, w.first ? 0 : 1, 0);
+        const int last = static_cast<int>((per * blockIdx.x + w.done + w.steps - 1) / per);
+        p.ws_units[w.unit(p)] = make_int4(static_cast<int>(blockIdx.x), last, w.first() ? 0 : 1, 0);
       }
       tc_fence_before();
     }
