@@ -144,6 +144,11 @@ __device__ __forceinline__ void tmem_wait_ld32(uint32_t* r) {
                  "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
                  "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
 }
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
+}
 // 16 consecutive fp32 columns of this thread's TMEM lane.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
   asm volatile(
@@ -962,32 +967,33 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
           }
           continue;
         }
-        if (!(ok = spin_bar(bar(kKFull + (t & 1)), (t >> 1) & 1, abort_flag))) break;
         if (!(ok = spin_bar(bar(kQFull + i), segs & 1, abort_flag))) break;
         ++segs;
-        tc_fence_after();
-        issue_s(t);
-        tc_commit(bar(kSFull + i));
-        tc_commit(bar(kKEmpty + (t & 1)));
-        for (int jj = 0; jj < count; ++jj, ++t, ++tq) {
-          const bool more = jj + 1 < count;
-          if (!(ok = spin_bar(bar(kVFull + (t & 1)), (t >> 1) & 1, abort_flag))) break;
-          if (!(ok = spin_bar(bar(kPHalf + i), tq & 1, abort_flag))) break;
-          tc_fence_after();
-          issue_pv(t, false, jj == 0);
-          if (more && !(ok = spin_bar(bar(kKFull + ((t + 1) & 1)), ((t + 1) >> 1) & 1, abort_flag))) break;
-          if (!(ok = spin_bar(bar(kPFull + i), tq & 1, abort_flag))) break;
-          tc_fence_after();
-          issue_pv(t, true, false);
-          if (more) {
-            issue_s(t + 1);
+        // Round jj: P V of tile jj, S of tile jj + 1 (t is tile jj + 1's).
+        for (int jj = -1; jj < count; ++jj) {
+          const int last = t - 1;  // tile jj's number
+          if (jj >= 0) {
+            if (!(ok = spin_bar(bar(kVFull + (last & 1)), (last >> 1) & 1, abort_flag))) break;
+#pragma unroll 1
+            for (int second = 0; second < 2; ++second) {
+              if (!(ok = spin_bar(bar((second ? kPFull : kPHalf) + i), tq & 1, abort_flag))) break;
+              tc_fence_after();
+              issue_pv(last, second, jj == 0 && !second);
+            }
+            if (!ok) break;
+            ++tq;
+          }
+          if (jj + 1 < count) {
+            if (!(ok = spin_bar(bar(kKFull + (t & 1)), (t >> 1) & 1, abort_flag))) break;
+            tc_fence_after();
+            issue_s(t);
             tc_commit(bar(kSFull + i));
-            tc_commit(bar(kVEmpty + (t & 1)));
-            tc_commit(bar(kKEmpty + ((t + 1) & 1)));
+            tc_commit(bar(kKEmpty + (t & 1)));
+            ++t;
           } else {
             tc_commit(bar(kOFinal + i));
-            tc_commit(bar(kVEmpty + (t & 1)));
           }
+          if (jj >= 0) tc_commit(bar(kVEmpty + (last & 1)));
         }
       }
       tc_commit(bar(kMmaDone));
@@ -1004,7 +1010,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
     const int turn = kTurn + 2 * (warp & 3);  // barrier turn + i: this pair's warp of tile i may go
     bool ok = true;
     for (bool more = w.begin(p, start, n_steps); ok && more; more = w.next(p)) {
-      if (qi == 1 && !w.two(p)) continue;
+      const bool two = w.two(p);
+      if (qi == 1 && !two) continue;
       // This thread's query row (rows of the K/V head), its token and its offset in q and out.
       auto q_row = [&] { return w.qb * kUnitRows + qi * kM + row; };
       auto row_at = [&](const int64_t member, const int64_t token_stride) {
@@ -1060,36 +1067,42 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
       for (int j = w.j0; j < w.j1; ++j, ++n_tiles) {
         if (!(ok = warp_spin(bar(kSFull + qi), n_tiles & 1, abort_flag))) break;
         tc_fence_after();
-        // Two passes over the scores in tensor memory, 32 columns at a time with the next 32 on their way:
-        // the row's maximum, then the probabilities.  The loops stay rolled: a sub-partition runs four
-        // roles' code side by side, and unrolled they wait for instructions more than for anything else.
-        const bool masked = j >= j_mask || any_bad;
-        const uint32_t bad = any_bad ? bad_pages(j * segs_tile, min((j + 1) * segs_tile, pages_seen)) : 0;
-        const int valid = lim - j * kTileKeys;
-        auto hide = [&](uint32_t* x, int first) {
+        // A tile of which the row does not see every key: -inf over the others, in tensor memory, so that
+        // the passes below need not know.
+        if (j >= j_mask || any_bad) {
+          const uint32_t bad = any_bad ? bad_pages(j * segs_tile, min((j + 1) * segs_tile, pages_seen)) : 0;
+          const int valid = lim - j * kTileKeys;
+#pragma unroll 1
+          for (int col = 0; col < 128; col += 16) {
+            uint32_t y[16];
+            tmem_ld16(s_addr + col, y);
+            tmem_wait_ld16(y);
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (first + i >= valid || ((bad >> ((first + i) >> shift)) & 1)) x[i] = __float_as_uint(-INFINITY);
-        };
+            for (int i = 0; i < 16; ++i)
+              if (col + i >= valid || ((bad >> ((col + i) >> shift)) & 1)) y[i] = __float_as_uint(-INFINITY);
+            tmem_st16(s_addr + col, y);
+          }
+          tmem_wait_st();
+        }
+        // Two passes over the scores in tensor memory, 32 columns at a time with the next 32 on their way:
+        // the row's maximum, then the probabilities.  The loops stay rolled: a sub-partition runs
+        // four roles' code side by side, and unrolled they wait for instructions more than for anything
+        // else (the 1.3B block call took 600 us with this loop unrolled).
         uint32_t xa[32], xb[32];
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         auto largest = [&](const uint32_t* y) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              mx[e] = max3(mx[e], __uint_as_float(y[i + 2 * e]), __uint_as_float(y[i + 2 * e + 1]));
+          for (int i = 0; i < 32; i += 2)
+            mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(y[i]), __uint_as_float(y[i + 1]));
         };
         tmem_ld32(s_addr, xa);
 #pragma unroll 1
         for (int col = 0; col < 128; col += 64) {
           tmem_wait_ld32(xa);
           tmem_ld32(s_addr + col + 32, xb);
-          if (masked) hide(xa, col);
           largest(xa);
           tmem_wait_ld32(xb);
           tmem_ld32(s_addr + ((col + 64) & 127), xa);  // the last one is the second pass's first
-          if (masked) hide(xb, col + 32);
           largest(xb);
         }
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
@@ -1106,7 +1119,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
           for (int c = 0; c < 8; ++c) {
             uint32_t o[16];
             tmem_ld16(o_addr + 16 * c, o);
-            tmem_wait_ld();
+            tmem_wait_ld16(o);
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
             tmem_st16(o_addr + 16 * c, o);
@@ -1116,7 +1129,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
         const f32x2 scale2 = f2_make(scale, scale), ref2 = f2_make(-ref, -ref);
         f32x2 sum[2] = {0, 0};
         // Tile 0's k-th turn follows tile 1's (k-1)-th, tile 1's k-th follows tile 0's k-th.
-        if (w.two(p)) {
+        if (two) {
           if (qi + n_turns > 0 && !(ok = warp_spin(bar(turn + qi), (n_turns - 1 + qi) & 1, abort_flag))) break;
           ++n_turns;
         }
@@ -1138,13 +1151,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
         for (int col = 0; col < 128; col += 64) {
           tmem_wait_ld32(xa);
           tmem_ld32(s_addr + col + 32, xb);
-          if (masked) hide(xa, col);
           exponentiate(xa, col >> 1);
           tmem_wait_ld32(xb);
           if (col == 0) tmem_ld32(s_addr + 64, xa);
-          if (masked) hide(xb, col + 32);
           exponentiate(xb, (col >> 1) + 16);
-          if (col != 0 && w.two(p) && lane == 0) bar_arrive(bar(turn + 1 - qi));
+          if (col != 0 && two && lane == 0) bar_arrive(bar(turn + 1 - qi));
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
@@ -1166,7 +1177,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
         for (int c = 0; c < 4; ++c) {
           uint32_t o[32];
           tmem_ld32(o_addr + 32 * c, o);
-          tmem_wait_ld();
+          tmem_wait_ld32(o);
           if (live) {
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
@@ -1187,7 +1198,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
         for (int c = 0; c < 4; ++c) {
           uint32_t o[32];
           tmem_ld32(o_addr + 32 * c, o);
-          tmem_wait_ld();
+          tmem_wait_ld32(o);
 #pragma unroll
           for (int v = 0; v < 4; ++v)
             asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + 32 * c + 8 * v), "r"(o[8 * v]),
