@@ -829,57 +829,72 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
     // Byte offset of part 0 (in write order) of key row 8 warp + r; part i is at dst0 ^ (16 i).
     const uint32_t dst0 = (c >> 1) * kHalf16 + (8 * warp + r) * 128 + ((((c & 1) * 4) ^ (right ? 2 : 0) ^ r) * 16);
     const uint32_t sel_a = right ? 0x3232 : 0x1010, sel_b = right ? 0x1010 : 0x3232;
-    // One packed tile (slot of ring position u) to the fp16 tile at `tile`, once `empty` has its phase.
-    // `seen`: keys of the tile that any row sees (V only: what a missing or unseen key holds must not
-    // reach the products even times a probability of 0, so its scale becomes 0).
-    auto expand = [&](int u, uint32_t tile, int empty, uint32_t parity, bool wait_empty, int seen) -> bool {
-      const int slot = u % kRawSlots;
-      if (!warp_spin(bar(kRawFull + slot), (u / kRawSlots) & 1, abort_flag)) return false;
-      if (wait_empty && !warp_spin(bar(empty), parity, abort_flag)) return false;
-      const uint32_t raw = sbase + kOffRaw + slot * kRawBytes;
-      const uint32_t there = *reinterpret_cast<volatile uint32_t*>(smem + kOffThere + 4 * slot);
-      const bool all = seen >= kTileKeys && there == (1u << (kTileKeys >> shift)) - 1;
-#pragma unroll 1
-      for (int i = 0; i < 4; ++i) {
-        const int key = 32 * i + 8 * warp + r, in_page = key & (page_rows - 1);
-        const uint32_t seg = raw + (key >> shift) * (page_rows * kKv4Row);
-        const uint32_t src = seg + in_page * 64 + c * 16 + (right ? 8 : 0);
-        uint32_t x[4];
-        asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(x[0]), "=r"(x[1]) : "r"(src));
-        asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(x[2]), "=r"(x[3]) : "r"(src ^ 8));
-        uint16_t two;
-        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(two) : "r"(seg + page_rows * 64 + in_page * 8 + c * 2));
-        uint32_t s2 = two;
-        if (!all && (key >= seen || !((there >> (key >> shift)) & 1))) s2 = 0;
-        const uint32_t sc = kv4_scales(s2);
-        const uint32_t sa = __byte_perm(sc, sc, sel_a), sb = __byte_perm(sc, sc, sel_b);
+    uint32_t from[4];  // of key i: offsets of its code chunk (low half) and scale pair (high half) in a slot
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          uint32_t o[4];
-          kv4_unpack(x[k], o);
-          const uint32_t f = k < 2 ? sa : sb;
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(tile + 32 * i * 128 + (dst0 ^ (16 * k))),
-                       "r"(h2_mul(o[0], f)), "r"(h2_mul(o[1], f)), "r"(h2_mul(o[2], f)), "r"(h2_mul(o[3], f))
-                       : "memory");
-        }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) bar_arrive(bar(kRawEmpty + slot));
-      return true;
-    };
-    int t = 0;
+    for (int i = 0; i < 4; ++i) {
+      const int key = 32 * i + 8 * warp + r, in_page = key & (page_rows - 1);
+      const uint32_t seg = (key >> shift) * (page_rows * kKv4Row);
+      from[i] = (seg + in_page * 64 + c * 16 + (right ? 8 : 0)) | ((seg + page_rows * 64 + in_page * 8 + c * 2) << 16);
+    }
+    const uint32_t every_page = (1u << (kTileKeys >> shift)) - 1;
+    int t = 0, slot = 0;
+    uint32_t slot_phase = 0;
     bool ok = true;
     for (bool more = w.begin(p, start, n_steps); ok && more; more = w.next(p)) {
-      for (int j = w.j0; j < w.j1; ++j, ++t) {
+      for (int j = w.j0; ok && j < w.j1; ++j, ++t) {
         const int st = t & 1;
-        const uint32_t parity = ((t >> 1) & 1) ^ 1;
-        if (!(ok = expand(2 * t, sbase + kOffK + st * kTile16, kKEmpty + st, parity, t >= 2, kTileKeys))) break;
-        if (lane == 0) bar_arrive(bar(kKFull + st));
-        if (!(ok = expand(2 * t + 1, sbase + kOffV + st * kTile16, kVEmpty + st, parity, t >= 2,
-                          w.lim_top - j * kTileKeys)))
-          break;
-        if (lane == 0) bar_arrive(bar(kVFull + st));
+        // K, then V (one copy of the code for both: see the softmax loops).
+#pragma unroll 1
+        for (int kv = 0; kv < 2; ++kv) {
+          if (!(ok = warp_spin(bar(kRawFull + slot), slot_phase, abort_flag))) break;
+          if (t >= 2 && !(ok = warp_spin(bar((kv ? kVEmpty : kKEmpty) + st), ((t >> 1) & 1) ^ 1, abort_flag))) break;
+          const uint32_t raw = sbase + kOffRaw + slot * kRawBytes;
+          const uint32_t tile = sbase + (kv ? kOffV : kOffK) + st * kTile16;
+          uint32_t x[4][4], s2[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t src = raw + (from[i] & 0xffffu);
+            asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(x[i][0]), "=r"(x[i][1]) : "r"(src));
+            asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(x[i][2]), "=r"(x[i][3]) : "r"(src ^ 8));
+            uint16_t two;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(two) : "r"(raw + (from[i] >> 16)));
+            s2[i] = two;
+          }
+          const uint32_t there = *reinterpret_cast<volatile uint32_t*>(smem + kOffThere + 4 * slot);
+          const int seen = w.lim_top - j * kTileKeys;
+          // What a missing or unseen key holds must not reach the products, even times a probability of 0.
+          if (seen < kTileKeys || there != every_page) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int key = 32 * i + 8 * warp + r;
+              if (key >= seen || !((there >> (key >> shift)) & 1)) s2[i] = 0;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t sc = kv4_scales(s2[i]);
+            const uint32_t sa = __byte_perm(sc, sc, sel_a), sb = __byte_perm(sc, sc, sel_b);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t o[4];
+              kv4_unpack(x[i][k], o);
+              const uint32_t f = k < 2 ? sa : sb;
+              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(tile + (dst0 ^ (16 * k)) + 32 * i * 128),
+                           "r"(h2_mul(o[0], f)), "r"(h2_mul(o[1], f)), "r"(h2_mul(o[2], f)), "r"(h2_mul(o[3], f))
+                           : "memory");
+            }
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            bar_arrive(bar(kRawEmpty + slot));
+            bar_arrive(bar((kv ? kVFull : kKFull) + st));
+          }
+          if (++slot == kRawSlots) {
+            slot = 0;
+            slot_phase ^= 1;
+          }
+        }
       }
     }
   } else if (warp >= 12) {
