@@ -44,11 +44,11 @@ struct Kv4Dev {
 // Validates `c` (host) and fills `d`; `rows` receives members * table_pages * page_rows.
 int kv4_check_cache(const ps_kv4_cache& c, Kv4Dev* d, int64_t* rows);  // ps_kv4_prep.cu
 
-// Page of a table entry's index, or -1 (counted) if the entry names no page of the pool.
-__device__ __forceinline__ int64_t kv4_page(const Kv4Dev& c, int64_t index) {
+// Page of a table entry's index, or -1 if the entry names no page of the pool (counted if `count`).
+__device__ __forceinline__ int64_t kv4_page(const Kv4Dev& c, int64_t index, bool count = true) {
   const int32_t page = c.table[index];  // an ordinary load: the kernel before may have written it
   if (static_cast<uint32_t>(page) < c.num_pages) return page;
-  atomicAdd(&g_kv4_counts[kKv4BadPages], 1u);
+  if (count) atomicAdd(&g_kv4_counts[kKv4BadPages], 1u);
   return -1;
 }
 
@@ -108,18 +108,26 @@ __device__ __forceinline__ uint32_t e2m1_of(const f32x2* y) {
   return r;
 }
 
+// A tensor scale t as the quantisation uses it.
+struct Kv4Scale {
+  float t, six, inv_six;  // t, 6 t, 1 / (6 t)
+};
+static inline Kv4Scale kv4_scale_of(float t) { return Kv4Scale{t, 6.f * t, 1.f / (6.f * t)}; }
+
 // Quantises 16 numbers x (8 pairs) whose largest magnitude is `top` (finite): the scale byte is
 // returned, the codes go to `codes`.  Both formats have so few bits that numbers do lie midway
-// between two of theirs, so both quotients have to be the correctly rounded ones: top / (6 t) is an
-// IEEE division (one per block); x / (scale t) is x times the reciprocal, corrected once by its own
-// remainder (Markstein's division, IBM J. Res. Dev. 34, 1990): two packed multiply-adds a pair.
-__device__ __forceinline__ uint32_t kv4_quantise(const f32x2* x, float top, float tensor_scale, float six_scale,
-                                                 uint2& codes) {
-  const uint32_t byte = e4m3_of(__fdiv_rn(top, six_scale));
+// between two of theirs, so both quotients, top / (6 t) and x / (scale t), have to be exact where they
+// are representable: each is the product with a reciprocal, corrected once by its own remainder
+// (Markstein's division, IBM J. Res. Dev. 34, 1990).  The remainder is exact, so a reciprocal that is
+// an ulp or two off leaves 2^-44 of the quotient before its rounding.
+__device__ __forceinline__ uint32_t kv4_quantise(const f32x2* x, float top, const Kv4Scale& scale, uint2& codes) {
+  const float q0 = __fmul_rn(top, scale.inv_six);
+  const uint32_t byte = e4m3_of(__fmaf_rn(__fmaf_rn(-q0, scale.six, top), scale.inv_six, q0));
   const uint32_t s2 = kv4_scales(byte);
-  const float scale = __half2float(__ushort_as_half(static_cast<unsigned short>(s2 & 0xffffu)));
-  const float step = __fmul_rn(scale, tensor_scale);
-  const float inv = step > 0.f ? __frcp_rn(step) : 0.f;
+  const float step = __fmul_rn(__half2float(__ushort_as_half(static_cast<unsigned short>(s2 & 0xffffu))), scale.t);
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(step));
+  inv = step > 0.f ? inv : 0.f;
   const f32x2 inv2 = f2_make(inv, inv), neg2 = f2_make(-step, -step);
   f32x2 y[8];
 #pragma unroll
@@ -129,6 +137,13 @@ __device__ __forceinline__ uint32_t kv4_quantise(const f32x2* x, float top, floa
   }
   codes = make_uint2(e2m1_of(y), e2m1_of(y + 4));
   return byte;
+}
+
+// max(|a|, |b|, |c|); NaN if one of them is.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 }  // namespace ps

@@ -50,7 +50,8 @@ struct PParams {
   const void* k_sink;
   int64_t q_stride, k_stride, v_stride, q_out_stride, k_pre_stride, k_sink_stride;
   Kv4Dev cache;
-  float k_six, v_six;  // 6 * tensor scale
+  Kv4Scale k_scale, v_scale;
+  int64_t page_bytes;  // of all heads
   float eps, cq, ck;   // row lengths of Q and K
   int32_t heads;
   int32_t tpt;         // threads per token (whole warps)
@@ -65,9 +66,9 @@ struct PParams {
 };
 static_assert(sizeof(PParams) <= 8192, "kernel parameters too large");
 
-constexpr int kMaxTpt = 320;      // threads per token: 40 heads a pass, three passes
-constexpr int kMaxBlocks = 3;     // blocks of each of q, k, v that a thread holds
-constexpr int max_blocks(int dtype) { return dtype == PS_BF16 ? kMaxBlocks : 2; }  // fp32 blocks take twice the registers
+constexpr int kMaxTpt = 320;      // threads per token: 40 heads a pass
+// Blocks of a role that a thread holds at most (fp32 blocks take twice the registers).
+constexpr int max_blocks(int dtype) { return dtype == PS_BF16 ? 5 : 3; }
 
 // 32 bytes as one load / store where the rows allow it.
 __device__ __forceinline__ void ld32(const void* p, uint32_t* w, bool wide) {
@@ -105,13 +106,6 @@ template <> struct Block<__nv_bfloat16> {
     w[j] = Pairs16<__nv_bfloat16>::pack_pair(lo, hi);
   }
   __device__ __forceinline__ static f32x2 round(f32x2 v) { return Pairs16<__nv_bfloat16>::round(v); }
-  // Bits of the largest magnitude as fp32 (infinities and NaN order above every finite number).
-  __device__ __forceinline__ static uint32_t top_bits(const uint32_t* w) {
-    uint32_t m = w[0] & 0x7fff7fffu;
-#pragma unroll
-    for (int j = 1; j < 8; ++j) m = __vmaxu2(m, w[j] & 0x7fff7fffu);
-    return max(m << 16, m & 0xffff0000u);
-  }
   // sum += x^2 in fp64.  A bf16's exponent and fraction bits moved to a double's high word, with the
   // exponent rebased (zero and subnormals read as up to 2^-126: their squares vanish beside eps).
   __device__ __forceinline__ static double add_squares(const uint32_t* w, double sum) {
@@ -149,12 +143,6 @@ template <> struct Block<float> {
     w[2 * j + 1] = __float_as_uint(hi);
   }
   __device__ __forceinline__ static f32x2 round(f32x2 v) { return v; }
-  __device__ __forceinline__ static uint32_t top_bits(const uint32_t* w) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) m = max(m, w[j] & 0x7fffffffu);
-    return m;
-  }
   __device__ __forceinline__ static double add_squares(const uint32_t* w, double sum) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
@@ -174,16 +162,18 @@ __device__ __forceinline__ void weights16(const void* w, bool w_f32, int off, f3
   for (int e = 0; e < 16; e += E) load_weight_pairs<T>(w, w_f32, off + e, out + e / 2);
 }
 
-// Quantises a block held in words of T into the cache row at `codes` / `scale`.
-template <typename T>
-__device__ __forceinline__ void put_block(uint32_t* w, float tensor_scale, float six, unsigned char* codes,
-                                          unsigned char* scale) {
-  float top = __uint_as_float(Block<T>::top_bits(w));
-  f32x2 x[8];
+// Quantises 16 numbers into the cache row at `codes` / `scale_byte`.
+__device__ __forceinline__ void put_block(f32x2* x, const Kv4Scale& scale, unsigned char* codes,
+                                          unsigned char* scale_byte) {
+  float top = 0.f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = Block<T>::pair(w, j);
-  const float most = 448.f * six;  // the largest number the cache holds
-  if (!(top <= most)) {            // rare: NaN becomes 0, everything larger saturates
+  for (int j = 0; j < 8; ++j) {
+    float a, b;
+    f2_split(x[j], a, b);
+    top = max3_abs(top, a, b);
+  }
+  const float most = 448.f * scale.six;  // the largest number the cache holds
+  if (!(top <= most)) {                  // rare: NaN becomes 0, everything larger saturates
     if (!(top < INFINITY)) atomicAdd(&g_kv4_counts[kKv4NonFinite], 1u);
     top = 0.f;
 #pragma unroll
@@ -199,13 +189,16 @@ __device__ __forceinline__ void put_block(uint32_t* w, float tensor_scale, float
     }
   }
   uint2 c;
-  const uint32_t byte = kv4_quantise(x, top, tensor_scale, six, c);
+  const uint32_t byte = kv4_quantise(x, top, scale, c);
   *reinterpret_cast<uint2*>(codes) = c;
-  *scale = static_cast<unsigned char>(byte);
+  *scale_byte = static_cast<unsigned char>(byte);
 }
 
+// The roles one after another -- V, K, Q -- so that a thread holds the raw blocks of two roles at most (K's
+// loads are in flight while V is quantised): registers, and with them the tokens an SM works on side by
+// side, bound this kernel before memory does.
 template <typename T, int NB, bool FULL>
-__global__ void __launch_bounds__(kMaxTpt) kv4_prep_kernel(const __grid_constant__ PParams p) {
+__global__ void __launch_bounds__(NB == 5 ? 256 : kMaxTpt, NB == 5 ? 2 : 1) kv4_prep_kernel(const __grid_constant__ PParams p) {
   using B = Block<T>;
   constexpr int W = B::kWords;
   __shared__ double part_k[kMaxTpt / 32];
@@ -229,177 +222,197 @@ __global__ void __launch_bounds__(kMaxTpt) kv4_prep_kernel(const __grid_constant
   const bool do_q = (flags & kQ) && !sink, do_v = (flags & kV) && !sink, do_k = (flags & kK) || sink;
   const bool norm_q = (flags & kNormQ) && !sink, norm_k = (flags & kNormK) && !sink;
   const bool pre = !FULL && (flags & kPre) && !sink;
+  // Head i of this thread, and its block's columns.
+  const int col0 = head0 * kKv4D + slice * 16, col_step = p.hstep * kKv4D;
+  auto has_q = [&](int i) { return head0 + i * p.hstep < p.heads; };
+  auto has_k = [&](int i) { return head0 + i * p.hstep < p.cache.kv_heads; };
 
   if (!p.early) pdl_wait();
-  uint32_t qw[NB][W], kw[NB][W], vw[NB][W];
-  const T* krow = sink ? static_cast<const T*>(p.k_sink) + row * p.k_sink_stride
-                       : static_cast<const T*>(p.k) + row * p.k_stride;
+  uint32_t vw[NB][W], xw[NB][W];  // xw: K's blocks, then Q's
+  if (active && do_v) {
+    const T* src = static_cast<const T*>(p.v) + row * p.v_stride + col0;
 #pragma unroll
-  for (int i = 0; i < NB; ++i) {
-    const int head = head0 + i * p.hstep;
-    const int off = head * kKv4D + slice * 16;
-#pragma unroll
-    for (int j = 0; j < W; ++j) qw[i][j] = kw[i][j] = vw[i][j] = 0;
-    if (active && do_q && head < p.heads) B::load(static_cast<const T*>(p.q) + row * p.q_stride + off, qw[i], p.wide);
-    if (active && head < p.cache.kv_heads) {
-      if (do_k) B::load(krow + off, kw[i], p.wide);
-      if (do_v) B::load(static_cast<const T*>(p.v) + row * p.v_stride + off, vw[i], p.wide);
-    }
+    for (int i = 0; i < NB; ++i)
+      if (has_k(i)) B::load(src + i * col_step, vw[i], p.wide);
   }
-  // Positions, the cache row and this thread's slice of the tables.
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int j = 0; j < W; ++j) xw[i][j] = 0;
+  if (active && do_k) {
+    const T* src = (sink ? static_cast<const T*>(p.k_sink) + row * p.k_sink_stride
+                         : static_cast<const T*>(p.k) + row * p.k_stride) + col0;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+      if (has_k(i)) B::load(src + i * col_step, xw[i], p.wide);
+  }
+  // Positions and the cache row.
   const int f = static_cast<int>(div_by(static_cast<uint32_t>(l), sq.hw_magic));
   const int rr = l - f * sq.hw;
   int ring = sq.ring_slot0 + f;
   if (ring >= sq.ring_frames) ring -= sq.ring_frames;
   const int64_t kv_row = sq.ring_row + static_cast<int64_t>(ring) * sq.hw + rr;
-  int64_t t0, t1, t2;
-  if (p.axes) {
-    const int hh = static_cast<int>(div_by(static_cast<uint32_t>(rr), sq.gw_magic));
-    t0 = sq.frame_offset + f;
-    t1 = hh;
-    t2 = rr - hh * sq.gw;
-  } else {
-    t0 = t1 = t2 = sq.table_row + l;
-  }
-  f32x2 cc[8], ss[8];
-  int64_t page = -1;
-  if (active) {
-    if (do_q || do_k) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int pair = slice * 8 + j;
-        const int64_t at = (pair < p.tp ? t0 : (pair < p.thp ? t1 : t2)) * kKv4D + 2 * pair;
-        cc[j] = __ldg(reinterpret_cast<const unsigned long long*>(p.cos + at));
-        ss[j] = __ldg(reinterpret_cast<const unsigned long long*>(p.sin + at));
-      }
-    }
-    if (do_k || do_v) page = kv4_page(p.cache, kv_row >> p.cache.shift);
-  }
-  pdl_trigger();
-  if (p.early) pdl_wait();
-
+  const int64_t page = active && (do_k || do_v) ? kv4_page(p.cache, kv_row >> p.cache.shift, lt == 0) : -1;
+  // The token's K row of this thread's first head; V's is `half` bytes further, the next head's `step`.
   const int in_page = static_cast<int>(kv_row & ((1 << p.cache.shift) - 1));
-  const int64_t half = p.cache.head_bytes >> 1;  // K's part of (page, head)
-  const int64_t code_off = in_page * 64 + slice * 8;
-  const int64_t scale_off = (static_cast<int64_t>(64) << p.cache.shift) + in_page * 8 + slice;
+  const int64_t half = p.cache.head_bytes >> 1, step = p.hstep * p.cache.head_bytes;
+  unsigned char* const base = p.cache.pages + page * p.page_bytes + head0 * p.cache.head_bytes;
+  const int code_off = in_page * 64 + slice * 8, scale_off = (64 << p.cache.shift) + in_page * 8 + slice;
+  if (p.early) pdl_wait();
   if (do_v && page >= 0) {
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      const int head = head0 + i * p.hstep;
-      if (head < p.cache.kv_heads) {
-        unsigned char* base = kv4_head(p.cache, page, head) + half;
-        put_block<T>(vw[i], p.cache.v_scale, p.v_six, base + code_off, base + scale_off);
-      }
-    }
-  }
-
-  // Row sums.
-  float sum_q = 0.f;
-  double sum_k = 0.0;
-  if (norm_q) {
-    f32x2 a = 0;
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const f32x2 x = B::pair(qw[i], j);
-        a = f2_fma(x, x, a);
-      }
-    float x, y;
-    f2_split(a, x, y);
-    sum_q = x + y;
-  }
-  if (norm_k) {
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-      if (head0 + i * p.hstep < p.cache.kv_heads) sum_k = B::add_squares(kw[i], sum_k);
-  }
-  if (flags & (kNormQ | kNormK)) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      sum_q += __shfl_xor_sync(0xffffffffu, sum_q, o);
-      sum_k += __shfl_xor_sync(0xffffffffu, sum_k, o);
-    }
-    if (p.tpt > 32) {  // one token per CTA: every thread gets here
-      if ((lt & 31) == 0) {
-        part_q[lt >> 5] = sum_q;
-        part_k[lt >> 5] = sum_k;
-      }
-      __syncthreads();
-      sum_q = 0.f;
-      sum_k = 0.0;
-      for (int i = 0; i < p.tpt >> 5; ++i) {
-        sum_q += part_q[i];
-        sum_k += part_k[i];
-      }
-    }
-  }
-  float ssq_k = static_cast<float>(sum_k);
-  if (sizeof(T) == 2 && norm_k && isinf(ssq_k)) {  // uniform over the token: was there a NaN?
-    bool nan = false;
-#pragma unroll
-    for (int i = 0; i < NB; ++i) nan |= B::has_nan(kw[i]);
-    nan = p.tpt > 32 ? __syncthreads_or(nan) : __any_sync(0xffffffffu, nan);
-    if (nan) ssq_k = NAN;
-  }
-  if (!active) return;
-  const float rq = rstd_of(sum_q, p.cq, p.eps), rk = rstd_of(ssq_k, p.ck, p.eps);
-  const f32x2 rq2 = f2_make(rq, rq), rk2 = f2_make(rk, rk);
-
-  if (do_k) {
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const int head = head0 + i * p.hstep;
-      const int off = head * kKv4D + slice * 16;
-      if (head >= p.cache.kv_heads) continue;
+      if (!has_k(i)) continue;
       f32x2 x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = B::pair(kw[i], j);
+      for (int j = 0; j < 8; ++j) x[j] = B::pair(vw[i], j);
+      unsigned char* const at = base + i * step + half;
+      put_block(x, p.v_scale, at + code_off, at + scale_off);
+    }
+  }
+
+  // This thread's slice of the rotation tables.
+  f32x2 cc[8], ss[8];
+  if (active && (do_q || do_k)) {
+    int64_t t0, t1, t2;
+    if (p.axes) {
+      const int hh = static_cast<int>(div_by(static_cast<uint32_t>(rr), sq.gw_magic));
+      t0 = sq.frame_offset + f;
+      t1 = hh;
+      t2 = rr - hh * sq.gw;
+    } else {
+      t0 = t1 = t2 = sq.table_row + l;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int pair = slice * 8 + j;
+      const int64_t at = (pair < p.tp ? t0 : (pair < p.thp ? t1 : t2)) * kKv4D + 2 * pair;
+      cc[j] = __ldg(reinterpret_cast<const unsigned long long*>(p.cos + at));
+      ss[j] = __ldg(reinterpret_cast<const unsigned long long*>(p.sin + at));
+    }
+  }
+
+  // K.
+  float rk = 1.f;
+  if (flags & kNormK) {
+    double sum = 0.0;
+    if (norm_k) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+        if (has_k(i)) sum = B::add_squares(xw[i], sum);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (p.tpt > 32) {  // one token per CTA: every thread gets here
+      if ((lt & 31) == 0) part_k[lt >> 5] = sum;
+      __syncthreads();
+      sum = 0.0;
+      for (int i = 0; i < p.tpt >> 5; ++i) sum += part_k[i];
+    }
+    float ssq = static_cast<float>(sum);
+    if (sizeof(T) == 2 && norm_k && isinf(ssq)) {  // uniform over the token: was there a NaN?
+      bool nan = false;
+#pragma unroll
+      for (int i = 0; i < NB; ++i) nan |= B::has_nan(xw[i]);
+      nan = p.tpt > 32 ? __syncthreads_or(nan) : __any_sync(0xffffffffu, nan);
+      if (nan) ssq = NAN;
+    }
+    rk = rstd_of(ssq, p.ck, p.eps);
+  }
+  if (active && do_k) {
+    const f32x2 r2 = f2_make(rk, rk);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      if (!has_k(i)) continue;
+      const int off = col0 + i * col_step;
+      f32x2 x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = B::pair(xw[i], j);
       if (norm_k) {
         f32x2 w[8];
         weights16<T>(p.wk, p.w_f32, off, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = B::round(f2_mul(f2_mul(x[j], rk2), w[j]));
+        for (int j = 0; j < 8; ++j) x[j] = B::round(f2_mul(f2_mul(x[j], r2), w[j]));
       }
       if (pre) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           float a, b;
           f2_split(x[j], a, b);
-          B::set(kw[i], j, a, b);
+          B::set(xw[i], j, a, b);
         }
-        B::store(static_cast<T*>(p.k_pre) + row * p.k_pre_stride + off, kw[i], p.wide);
+        B::store(static_cast<T*>(p.k_pre) + row * p.k_pre_stride + off, xw[i], p.wide);
       }
       if (page >= 0) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           float a, b;
           rotate_f2(x[j], cc[j], ss[j], a, b);
-          B::set(kw[i], j, a, b);
+          x[j] = B::round(f2_make(a, b));  // what the ring would hold
         }
-        unsigned char* base = kv4_head(p.cache, page, head);
-        put_block<T>(kw[i], p.cache.k_scale, p.k_six, base + code_off, base + scale_off);
+        unsigned char* const at = base + i * step;
+        put_block(x, p.k_scale, at + code_off, at + scale_off);
       }
     }
   }
-  if (do_q) {
+
+  // Q.
+  if (!(flags & kQ)) {
+    pdl_trigger();
+    return;
+  }
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const int head = head0 + i * p.hstep;
-      const int off = head * kKv4D + slice * 16;
-      if (head >= p.heads) continue;
-      f32x2 w[8];
-      if (norm_q) weights16<T>(p.wq, p.w_f32, off, w);
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int j = 0; j < W; ++j) xw[i][j] = 0;
+  if (active && do_q) {
+    const T* src = static_cast<const T*>(p.q) + row * p.q_stride + col0;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+      if (has_q(i)) B::load(src + i * col_step, xw[i], p.wide);
+  }
+  pdl_trigger();  // every load is in flight: a dependent launch may be scheduled
+  float rq = 1.f;
+  if (flags & kNormQ) {
+    f32x2 a = 0;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        f32x2 x = B::pair(qw[i], j);
-        if (norm_q) x = B::round(f2_mul(f2_mul(x, rq2), w[j]));
-        float a, b;
-        rotate_f2(x, cc[j], ss[j], a, b);
-        B::set(qw[i], j, a, b);
+        const f32x2 x = B::pair(xw[i], j);
+        a = f2_fma(x, x, a);
       }
-      B::store(static_cast<T*>(p.q_out) + row * p.q_out_stride + off, qw[i], p.wide);
+    float x, y;
+    f2_split(a, x, y);
+    float sum = x + y;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (p.tpt > 32) {
+      if ((lt & 31) == 0) part_q[lt >> 5] = sum;
+      __syncthreads();
+      sum = 0.f;
+      for (int i = 0; i < p.tpt >> 5; ++i) sum += part_q[i];
     }
+    rq = rstd_of(sum, p.cq, p.eps);
+  }
+  if (!active || !do_q) return;
+  const f32x2 r2 = f2_make(rq, rq);
+  T* const dst = static_cast<T*>(p.q_out) + row * p.q_out_stride;
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
+    if (!has_q(i)) continue;
+    const int off = col0 + i * col_step;
+    f32x2 w[8];
+    if (norm_q) weights16<T>(p.wq, p.w_f32, off, w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      f32x2 x = B::pair(xw[i], j);
+      if (norm_q) x = B::round(f2_mul(f2_mul(x, r2), w[j]));
+      float a, b;
+      rotate_f2(x, cc[j], ss[j], a, b);
+      B::set(xw[i], j, a, b);
+    }
+    B::store(dst + off, xw[i], p.wide);
   }
 }
 
@@ -507,17 +520,16 @@ static bool wide32(const void* p, int64_t stride, int es) {
   return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 31u) == 0 && (stride * es) % 32 == 0);
 }
 
-// Blocks per thread and threads per token: the split of the larger head count that leaves the fewest
-// threads without a block, and of equal ones the one with most blocks a thread (the per-token work --
-// decode, tables, row sums -- is then shared by the fewest warps).
+// Blocks per thread and warps per token for the larger head count, by the instructions a token costs (counted
+// on a B200, bf16): about 500 a warp (decode, tables, row sums) and 640 for a block of each of Q, K and V.
+// 40 heads: five blocks and two warps 150 us, two blocks and five warps 162 us (12 480 tokens).
 static void choose_split(int heads, int max_nb, int* nb, int* warps) {
-  double best = -1;
+  int best = 0;
   for (int n = 1; n <= max_nb; ++n) {
     const int w = (heads + 4 * n - 1) / (4 * n);
-    if (w * 32 > kMaxTpt) continue;
-    const double used = static_cast<double>(heads) / (w * 4 * n);
-    if (used >= best - 0.02) {
-      best = used > best ? used : best;
+    const int cost = w * (500 + 640 * n);
+    if (w * 32 <= kMaxTpt && (best == 0 || cost < best)) {
+      best = cost;
       *nb = n;
       *warps = w;
     }
@@ -541,7 +553,7 @@ static int build_prep(const ps_kv4_prep_args* a, PPlan* plan) {
   int rc = kv4_check_cache(a->cache, &p.cache, &cache_rows);
   if (rc) return rc;
   const int hk = a->cache.kv_heads;
-  const int max_heads = kMaxTpt / 8 * max_blocks(a->dtype);
+  const int max_heads = a->dtype == PS_BF16 ? 120 : 80;
   if (a->heads < 1 || a->heads > max_heads || hk > max_heads)
     return fail(PS_ERR_UNSUPPORTED, "heads=%d kv_heads=%d: 1..%d", a->heads, hk, max_heads);
   const int es = a->dtype == PS_BF16 ? 2 : 4;
@@ -649,8 +661,9 @@ static int build_prep(const ps_kv4_prep_args* a, PPlan* plan) {
   p.cos = a->cos; p.sin = a->sin; p.q_out = a->q_out; p.k_pre = a->k_pre; p.k_sink = a->k_sink;
   p.q_stride = a->q_stride; p.k_stride = a->k_stride; p.v_stride = a->v_stride;
   p.q_out_stride = a->q_out_stride; p.k_pre_stride = a->k_pre_stride; p.k_sink_stride = a->k_sink_stride;
-  p.k_six = 6.f * a->cache.k_scale;
-  p.v_six = 6.f * a->cache.v_scale;
+  p.k_scale = kv4_scale_of(a->cache.k_scale);
+  p.v_scale = kv4_scale_of(a->cache.v_scale);
+  p.page_bytes = p.cache.head_bytes * hk;
   p.eps = a->eps;
   p.cq = static_cast<float>(C);
   p.ck = static_cast<float>(Ck);
@@ -666,7 +679,11 @@ static int build_prep(const ps_kv4_prep_args* a, PPlan* plan) {
   plan->dtype = a->dtype;
   int warps = 1;
   plan->nb = 1;
-  choose_split(a->heads > hk ? a->heads : hk, max_blocks(a->dtype), &plan->nb, &warps);
+  // A launch that one block a thread does not fill the GPU with (eight warps an SM) is bound by the time
+  // of a token, not by throughput: then one block a thread (8 tokens of 12 heads: 3.2 us against 5.7).
+  const int most = a->heads > hk ? a->heads : hk;
+  const bool few = total * ((most + 3) / 4) <= 148 * 8;
+  choose_split(most, few && (most + 3) / 4 * 32 <= kMaxTpt ? 1 : max_blocks(a->dtype), &plan->nb, &warps);
   p.tpt = warps * 32;
   p.hstep = warps * 4;
   p.tokens_cta = warps == 1 ? 2 : 1;
@@ -691,15 +708,20 @@ static cudaError_t launch_pdl(void (*fn)(P), const P& params, int64_t blocks, in
   return cudaLaunchKernelEx(&cfg, fn, params);
 }
 
+template <typename T, int NB>
+static void (*prep_fn(bool full))(PParams) {
+  return full ? kv4_prep_kernel<T, NB, true> : kv4_prep_kernel<T, NB, false>;
+}
 static void (*prep_fn(int dtype, int nb, bool full))(PParams) {
-  if (dtype == PS_F32) {
-    if (nb == 1) return full ? kv4_prep_kernel<float, 1, true> : kv4_prep_kernel<float, 1, false>;
-    return full ? kv4_prep_kernel<float, 2, true> : kv4_prep_kernel<float, 2, false>;
+  if (dtype == PS_F32)
+    return nb == 1 ? prep_fn<float, 1>(full) : nb == 2 ? prep_fn<float, 2>(full) : prep_fn<float, 3>(full);
+  switch (nb) {
+    case 1: return prep_fn<__nv_bfloat16, 1>(full);
+    case 2: return prep_fn<__nv_bfloat16, 2>(full);
+    case 3: return prep_fn<__nv_bfloat16, 3>(full);
+    case 4: return prep_fn<__nv_bfloat16, 4>(full);
+    default: return prep_fn<__nv_bfloat16, 5>(full);
   }
-  typedef __nv_bfloat16 T;
-  if (nb == 1) return full ? kv4_prep_kernel<T, 1, true> : kv4_prep_kernel<T, 1, false>;
-  if (nb == 2) return full ? kv4_prep_kernel<T, 2, true> : kv4_prep_kernel<T, 2, false>;
-  return full ? kv4_prep_kernel<T, 3, true> : kv4_prep_kernel<T, 3, false>;
 }
 
 static int build_read(const ps_kv4_read_args* a, RParams* p) {
