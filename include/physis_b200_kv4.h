@@ -105,8 +105,8 @@ typedef struct ps_kv4_read_args {
 /* Which kernel ps_attention_kv4 runs. */
 typedef enum ps_kv4_kernel {
   PS_KV4_AUTO = 0,
-  PS_KV4_ROWS = 1, /* up to 16 query rows a K/V head at a time, bound by reading the cache */
-  PS_KV4_TILES = 2 /* tiles of 128 query rows on the tcgen05 tensor cores */
+  PS_KV4_ROWS = 1, /* 8 query rows of a K/V head at a time, bound by reading the cache */
+  PS_KV4_TILES = 2 /* 256 query rows of a K/V head at a time on the tcgen05 tensor cores */
 } ps_kv4_kernel;
 
 /* Arguments of ps_attention_kv4.  Query row t of member b, head h starts at

@@ -76,7 +76,7 @@ __device__ __forceinline__ float row_power(float top, float& back) {
 }
 
 // ---------------------------------------------------------------------------------------
-// rows kernel: up to 8 * NT query rows of a K/V head
+// rows kernel: up to 8 query rows of a K/V head
 // ---------------------------------------------------------------------------------------
 // Bound: HBM, 144 bytes a (key, K/V head).  One CTA takes a (member, K/V head, row block) and one
 // chunk of its keys.  A producer warp brings 128-key tiles into a ring of shared-memory stages, one
@@ -98,6 +98,7 @@ __device__ __forceinline__ float row_power(float top, float& back) {
 constexpr int kRowWarps = 4;
 constexpr int kRowThreads = 32 * (kRowWarps + 1);
 constexpr int kStages = 3;
+constexpr int kBlockRows = 8;   // query rows of a CTA
 
 __device__ __forceinline__ int key_of(int i) { return (0x65742130u >> (4 * i)) & 7; }  // 0 3 1 2 4 7 5 6
 
@@ -166,9 +167,8 @@ struct RowsShared {
   int abort;
 };
 
-template <int NT>
 __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_constant__ AParams p) {
-  constexpr int R = 8 * NT;
+  constexpr int R = kBlockRows;
   extern __shared__ unsigned char smem_raw[];
   RowsShared& sh = *reinterpret_cast<RowsShared*>(
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127)));
@@ -209,25 +209,32 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
   if (warp == kRowWarps) {
     // ------------------------------- producer -------------------------------
     int t = 0;
+    // Lane i: table entry of the tile's page i, a tile ahead (unconditional loads, so that nothing waits for
+    // them before they are used).
+    auto seen = [&](int j) { return lane < segs && j * kTileKeys + (lane << shift) < lim_top; };
+    auto entry_of = [&](int j) {
+      const int64_t i = seen(j) ? ((static_cast<int64_t>(j) * kTileKeys) >> shift) + lane : 0;
+      uint32_t x;
+      asm volatile("ld.global.u32 %0, [%1];" : "=r"(x) : "l"(p.cache.table + b * p.cache.table_pages + i));
+      return x;
+    };
+    uint32_t entry = entry_of(j0);
     for (int j = j0; j < j1; ++j, ++t) {
       const int s = t % kStages;
-      // The page first: its latency overlaps the wait for the stage.
-      int64_t page = -1;
-      const int64_t first = (static_cast<int64_t>(j) << 7 >> shift) + lane;
-      const bool mine = lane < segs && (first << shift) < lim_top;
-      if (mine) page = kv4_page(p.cache, b * p.cache.table_pages + first);
-      const unsigned valid = __ballot_sync(0xffffffffu, page >= 0);
+      const bool mine = seen(j), valid_page = mine && entry < p.cache.num_pages;
+      if (mine && !valid_page) atomicAdd(&g_kv4_counts[kKv4BadPages], 1u);
+      const unsigned char* src = kv4_head(p.cache, valid_page ? entry : 0, h);
+      entry = entry_of(j + 1);
+      const unsigned valid = __ballot_sync(0xffffffffu, valid_page);
       const unsigned wanted = __ballot_sync(0xffffffffu, mine);
-      if (t >= kStages &&
-          !warp_wait(saddr(&sh.empty[s]), ((t / kStages) & 1) ^ 1, abort_flag, lane))
-        break;
+      if (t >= kStages && !warp_wait(saddr(&sh.empty[s]), ((t / kStages) & 1) ^ 1, abort_flag, lane)) break;
       const uint32_t bar = saddr(&sh.full[s]);
       if (lane == 0) {
         sh.bad[s] = wanted & ~valid;
         bar_expect_tx(bar, __popc(valid) * seg_bytes);
       }
       __syncwarp();
-      if (page >= 0) bulk_load(saddr(sh.stage[s]) + lane * seg_bytes, kv4_head(p.cache, page, h), seg_bytes, bar);
+      if (valid_page) bulk_load(saddr(sh.stage[s]) + lane * seg_bytes, src, seg_bytes, bar);
     }
     pdl_trigger();
     // Every copy has landed before the CTA may exit (the consumers have waited for theirs unless the
@@ -240,25 +247,22 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
 
   // ------------------------------- consumers -------------------------------
   const int g = lane >> 2, c = lane & 3;
-  float o[NT][8][4];
-  float m[NT][2], l[NT][2];
-#pragma unroll
-  for (int x = 0; x < NT; ++x) {
+  float o[8][4];
+  float m[2], l[2];
+  {
 #pragma unroll
     for (int t = 0; t < 8; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[x][t][e] = 0.f;
-    m[x][0] = m[x][1] = -INFINITY;
-    l[x][0] = l[x][1] = 0.f;
+      for (int e = 0; e < 4; ++e) o[t][e] = 0.f;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
   }
   if (warp < kRowWarps) {
     // Q: query row g of each group of eight, elements 32c .. 32c+31, scaled to fp16.
-    uint32_t qf[NT][16];
-    float qs[NT][2];   // score scale of the query rows 2c, 2c + 1
-    int lim[NT][2];
-#pragma unroll
-    for (int x = 0; x < NT; ++x) {
-      const int r = row0 + 8 * x + g;
+    uint32_t qf[16];
+    float qs[2];   // score scale of the query rows 2c, 2c + 1
+    {
+      const int r = row0 + g;
       uint4 w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = make_uint4(0, 0, 0, 0);
@@ -280,13 +284,9 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
       const float power = row_power(__uint_as_float(top), back);
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        qf[x][i] = h2_pack(__uint_as_float(v[i] << 16) * power, __uint_as_float(v[i] & 0xffff0000u) * power);
+        qf[i] = h2_pack(__uint_as_float(v[i] << 16) * power, __uint_as_float(v[i] & 0xffff0000u) * power);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        qs[x][e] = __shfl_sync(0xffffffffu, back, (2 * c + e) * 4) * p.scale_log2;
-        const int rq = row0 + 8 * x + 2 * c + e;
-        lim[x][e] = rq < row_end ? token_limit(p, n, rq / p.group) : n;
-      }
+      for (int e = 0; e < 2; ++e) qs[e] = __shfl_sync(0xffffffffu, back, (2 * c + e) * 4) * p.scale_log2;
     }
     const int kg = key_of(g);                                   // K rows of this lane: kg, kg + 8
     const int v0 = key_of(2 * c), v1 = key_of(2 * c + 1);       // V rows: v0, v1, v0 + 8, v1 + 8
@@ -300,11 +300,15 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
       if (!warp_wait(saddr(&sh.full[s]), (t / kStages) & 1, abort_flag, lane)) break;
       const uint32_t bad = *reinterpret_cast<volatile uint32_t*>(&sh.bad[s]);
       const bool masked = (j + 1) * kTileKeys > lim_low || bad != 0;
-      float acc[2][NT][4];
-      // S^T of this warp's 32 keys, two steps of 16.
+      // This warp's 32 keys, two groups of 16 side by side: a group's products are chains of dependent MMAs,
+      // and with few warps it is their latency that counts (one after the other: 16 x 1 rows over 34 320
+      // keys 255 us instead of 214, with a fourth CTA an SM).
+      constexpr int U = 2;
+      const int key0 = warp * 32;
+      float acc[U][4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int key = warp * 32 + u * 16;
+      for (int u = 0; u < U; ++u) {  // S^T
+        const int key = key0 + 16 * u;
         const unsigned char* base = sh.stage[s] + (key >> shift) * seg_bytes;
         const int in0 = key & (page_rows - 1);
         const unsigned char* kc = base + in0 * 64 + k_codes;
@@ -315,10 +319,9 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
         const uint32_t s1 = kv4_scales(*reinterpret_cast<const uint16_t*>(ksc + 8 * 8));
         const uint32_t s0l = __byte_perm(s0, s0, 0x1010), s0h = __byte_perm(s0, s0, 0x3232);
         const uint32_t s1l = __byte_perm(s1, s1, 0x1010), s1h = __byte_perm(s1, s1, 0x3232);
+        float part[4];  // the second half of the head dimension: a chain of its own
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[u][x][e] = 0.f;
+        for (int e = 0; e < 4; ++e) acc[u][e] = part[e] = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           uint32_t x0[4], x1[4];
@@ -329,66 +332,70 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
           for (int k = 0; k < 2; ++k) {
             const uint32_t a[4] = {h2_mul(x0[2 * k], sa), h2_mul(x1[2 * k], sb), h2_mul(x0[2 * k + 1], sa),
                                    h2_mul(x1[2 * k + 1], sb)};
-#pragma unroll
-            for (int x = 0; x < NT; ++x) mma16816(acc[u][x], a, qf[x][4 * i + 2 * k], qf[x][4 * i + 2 * k + 1]);
+            mma16816(k ? part : acc[u], a, qf[4 * i + 2 * k], qf[4 * i + 2 * k + 1]);
           }
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[u][e] = (acc[u][e] + part[e]) * qs[e & 1];
       }
       // Scores in log2 units; what a row does not see becomes -inf.
+      if (masked) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int lim = token_limit(p, n, min(row0 + 2 * c + e, p.rows - 1) / p.group) - j * kTileKeys;
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int in_tile = key0 + 16 * u + kg + 8 * k;
+              if (in_tile >= lim || ((bad >> (in_tile >> shift)) & 1)) acc[u][e + 2 * k] = -INFINITY;
+            }
+        }
+      }
       bool grow = false;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            acc[u][x][e] *= qs[x][e & 1];
-            if (masked) {
-              const int in_tile = warp * 32 + u * 16 + kg + (e >> 1) * 8;
-              if (j * kTileKeys + in_tile >= lim[x][e & 1] || ((bad >> (in_tile >> shift)) & 1)) acc[u][x][e] = -INFINITY;
-            }
-            grow |= acc[u][x][e] > m[x][e & 1] + 8.f;
-          }
+        for (int e = 0; e < 4; ++e) grow |= acc[u][e] > m[e & 1] + 8.f;
       // The reference of a row moves only when a score exceeds it by more than 8 (probabilities are
       // exact for any reference; fp16 holds them up to 2^8 with the same relative rounding).
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
+        for (int e = 0; e < 2; ++e) {
+          float top = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(fmaxf(acc[0][x][e], acc[0][x][e + 2]), fmaxf(acc[1][x][e], acc[1][x][e + 2]));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            const float next = fmaxf(m[x][e], top);
-            const float alpha = next == -INFINITY ? 1.f : fast_exp2(m[x][e] - next);
-            m[x][e] = next;
-            l[x][e] *= alpha;
+          for (int u = 0; u < U; ++u) top = fmaxf(top, fmaxf(acc[u][e], acc[u][e + 2]));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          const float next = fmaxf(m[e], top);
+          const float alpha = next == -INFINITY ? 1.f : fast_exp2(m[e] - next);
+          m[e] = next;
+          l[e] *= alpha;
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              o[x][q][e] *= alpha;
-              o[x][q][e + 2] *= alpha;
-            }
+          for (int q = 0; q < 8; ++q) {
+            o[q][e] *= alpha;
+            o[q][e + 2] *= alpha;
           }
+        }
       }
-      uint32_t pb[2][NT][2];
+      uint32_t pb[U][2];
+      {
+        const float r0 = m[0] == -INFINITY ? 0.f : m[0], r1 = m[1] == -INFINITY ? 0.f : m[1];
 #pragma unroll
-      for (int x = 0; x < NT; ++x) {
-        const float r0 = m[x][0] == -INFINITY ? 0.f : m[x][0], r1 = m[x][1] == -INFINITY ? 0.f : m[x][1];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float p0 = fast_exp2(acc[u][x][0] - r0), p1 = fast_exp2(acc[u][x][1] - r1);
-          const float p2 = fast_exp2(acc[u][x][2] - r0), p3 = fast_exp2(acc[u][x][3] - r1);
-          l[x][0] += p0 + p2;
-          l[x][1] += p1 + p3;
-          pb[u][x][0] = transpose8(h2_pack(p0, p1));
-          pb[u][x][1] = transpose8(h2_pack(p2, p3));
+        for (int u = 0; u < U; ++u) {
+          const float p0 = fast_exp2(acc[u][0] - r0), p1 = fast_exp2(acc[u][1] - r1);
+          const float p2 = fast_exp2(acc[u][2] - r0), p3 = fast_exp2(acc[u][3] - r1);
+          l[0] += p0 + p2;
+          l[1] += p1 + p3;
+          pb[u][0] = transpose8(h2_pack(p0, p1));
+          pb[u][1] = transpose8(h2_pack(p2, p3));
         }
       }
       // O^T += V^T P^T.
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int key = warp * 32 + u * 16;
+      for (int u = 0; u < U; ++u) {
+        const int key = key0 + 16 * u;
         const unsigned char* base = sh.stage[s] + (key >> shift) * seg_bytes;
         const int in0 = key & (page_rows - 1);
         uint2 w[4];
@@ -420,8 +427,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const uint32_t a[4] = {h2_mul(al[i], sa), h2_mul(ah[i], sa), h2_mul(bl[i], sb), h2_mul(bh[i], sb)};
-#pragma unroll
-            for (int x = 0; x < NT; ++x) mma16816(o[x][half * 4 + i], a, pb[u][x][0], pb[u][x][1]);
+            mma16816(o[half * 4 + i], a, pb[u][0], pb[u][1]);
           }
         }
       }
@@ -430,11 +436,9 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
     }
     // The rows' sums over the lanes that share them.
 #pragma unroll
-    for (int x = 0; x < NT; ++x)
+    for (int e = 0; e < 2; ++e)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l[x][e] += __shfl_xor_sync(0xffffffffu, l[x][e], d);
+      for (int d = 4; d < 32; d <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
   }
   // The four warps' results meet in the stages' memory: no copy is in flight any more.
   __syncthreads();
@@ -444,17 +448,15 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
   static_assert((kRowWarps * R * kStride + 2 * kRowWarps * R) * 4 <= kStages * kTileBytes, "merge buffer");
   if (warp < kRowWarps) {
 #pragma unroll
-    for (int x = 0; x < NT; ++x)
+    for (int e = 0; e < 2; ++e) {
+      const int r = 2 * c + e;
+      float* dst = part + (warp * R + r) * kStride + 16 * g;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = 8 * x + 2 * c + e;
-        float* dst = part + (warp * R + r) * kStride + 16 * g;
-#pragma unroll
-        for (int q = 0; q < 8; q += 2)
-          *reinterpret_cast<float4*>(dst + 2 * q) =
-              make_float4(o[x][q][e], o[x][q][e + 2], o[x][q + 1][e], o[x][q + 1][e + 2]);
-        if (g == 0) stat[warp * R + r] = make_float2(m[x][e], l[x][e]);
-      }
+      for (int q = 0; q < 8; q += 2)
+        *reinterpret_cast<float4*>(dst + 2 * q) =
+            make_float4(o[q][e], o[q][e + 2], o[q + 1][e], o[q + 1][e + 2]);
+      if (g == 0) stat[warp * R + r] = make_float2(m[e], l[e]);
+    }
   }
   __syncthreads();
   if (warp == kRowWarps) return;
@@ -1362,15 +1364,24 @@ static int build_attn(const ps_kv4_attn_args* a, APlan* plan, bool host_only) {
   const int64_t rows = static_cast<int64_t>(a->q_tokens) * p.group;
   if (rows > (1 << 30)) return fail(PS_ERR_UNSUPPORTED, "%lld query rows of a K/V head", (long long)rows);
   p.rows = static_cast<int32_t>(rows);
-  // The rows kernel reads the cache once per 16 query rows, the tiles kernel once per 256 but takes a
-  // whole 128-row tile's time for them.
-  plan->kernel = a->kernel != PS_KV4_AUTO ? a->kernel : (rows > 32 ? PS_KV4_TILES : PS_KV4_ROWS);
-  const bool tiles_kernel = plan->kernel == PS_KV4_TILES;
-  plan->block_rows = tiles_kernel ? kUnitRows : (rows <= 8 ? 8 : 16);
-  p.row_blocks = (p.rows + plan->block_rows - 1) / plan->block_rows;
-  p.units = a->cache.members * hk * p.row_blocks;
   const int tiles = (a->kv_tokens + kTileKeys - 1) / kTileKeys;
   const int sms = host_only ? 148 : sm_count();
+  plan->kernel = a->kernel;
+  if (plan->kernel == PS_KV4_AUTO) {
+    // The rows kernel passes over the keys once per 8 query rows, 0.62 us a 128-key tile on an SM; the tiles
+    // kernel once per 256 rows, about 2.2 us, and it takes 13 us to start and finish against 6 (measured).
+    // Per K/V head they meet between 24 and 32 rows on long windows (12 heads over 34 320 keys: 24 rows 48
+    // us against 68, 32 rows 60 against 68, 64 rows 112 against 70) and past 128 on short ones (1 024 keys:
+    // 15 us against 16).
+    const double heads_tiles = static_cast<double>(a->cache.members) * hk * tiles / sms;
+    const double rows_us = 6 + 0.62 * heads_tiles * ((rows + kBlockRows - 1) / kBlockRows);
+    const double tiles_us = 13 + 2.2 * heads_tiles * ((rows + kUnitRows - 1) / kUnitRows);
+    plan->kernel = rows_us <= tiles_us ? PS_KV4_ROWS : PS_KV4_TILES;
+  }
+  const bool tiles_kernel = plan->kernel == PS_KV4_TILES;
+  plan->block_rows = tiles_kernel ? kUnitRows : kBlockRows;
+  p.row_blocks = (p.rows + plan->block_rows - 1) / plan->block_rows;
+  p.units = a->cache.members * hk * p.row_blocks;
   const double scale = a->scale > 0.f ? a->scale : 1.0 / sqrt(static_cast<double>(kKv4D));
   p.scale_log2 = static_cast<float>(scale * a->cache.k_scale * 1.4426950408889634);
   if (p.units > (1 << 26)) return fail(PS_ERR_UNSUPPORTED, "%lld units of work", (long long)p.units);
@@ -1475,9 +1486,8 @@ extern "C" int32_t ps_attention_kv4(const ps_kv4_attn_args* args, void* stream) 
     return PS_OK;
   }
   const int smem = static_cast<int>(sizeof(ps::RowsShared)) + 128;
-  auto fn = plan.block_rows == 8 ? ps::kv4_rows_kernel<1> : ps::kv4_rows_kernel<2>;
-  cudaError_t err = ps::allow_smem(reinterpret_cast<const void*>(fn), smem);
-  if (err == cudaSuccess) err = ps::launch(fn, p.units * p.chunks, ps::kRowThreads, smem, s, p);
+  cudaError_t err = ps::allow_smem(reinterpret_cast<const void*>(ps::kv4_rows_kernel), smem);
+  if (err == cudaSuccess) err = ps::launch(ps::kv4_rows_kernel, p.units * p.chunks, ps::kRowThreads, smem, s, p);
   if (err == cudaSuccess && p.chunks > 1) {
     const int64_t rows = p.units / p.row_blocks * p.rows;
     err = ps::launch(ps::kv4_combine_kernel, (rows + 3) / 4, 128, 0, s, p, plan.block_rows);

@@ -696,6 +696,7 @@ _READ4 = struct.Struct("=iiqq" + "Qqq" * 2 + _KV4_CACHE)
 _ATTN4_HEAD = "=4if3i" + "Qqq" * 2 + "Q"
 _ATTN4 = struct.Struct(_ATTN4_HEAD + "Qq" + _KV4_CACHE)
 _ATTN4_WORKSPACE = struct.calcsize(_ATTN4_HEAD)
+_ATTN4_NEED: dict[tuple, int] = {}   # workspace bytes by the shape of a call
 
 
 def kv4_pages(num_pages: int, kv_heads: int, page_rows: int = 128, device=None) -> torch.Tensor:
@@ -913,23 +914,25 @@ def read_kv4(pages: torch.Tensor, table: torch.Tensor, tokens: int, *, row0: int
     device_index, members, _, cache = _kv4_cache(pages, table, k_scale, v_scale)
     C = pages.shape[1] * KV4_HEAD_DIM
     tokens, row0 = int(tokens), int(row0)
-    if tokens < 0:
-        raise PrepError(f"tokens={tokens}")
     dtype = next((t.dtype for t in (k_out, v_out) if t is not None), dtype)
     code = _DEVICE_DTYPES.get(dtype)
     if code is None:
         raise PrepError(f"unsupported dtype {dtype}: the kernels write bfloat16 or float32")
-    if k_out is None:
-        k_out = torch.empty(members, tokens, C, dtype=dtype, device=pages.device)
-    if v_out is None:
-        v_out = torch.empty(members, tokens, C, dtype=dtype, device=pages.device)
-    strides = []
+    if tokens < 0:
+        raise PrepError(f"tokens={tokens}")
+    outs, strides = [], []
     for name, t in (("k_out", k_out), ("v_out", v_out)):
+        if t is None:
+            outs.append(torch.empty(members, tokens, C, dtype=dtype, device=pages.device))
+            strides.append((tokens * C, C))
+            continue
         if t.dtype is not dtype or t.get_device() != device_index:
             raise PrepError(f"{name} is {t.dtype} on {t.device}, expected {dtype} on {pages.device}")
         if t.shape[0] != members or t.shape[1] != tokens:
             raise PrepError(f"{name} must be [{members}, {tokens}, {C}], got {tuple(t.shape)}")
+        outs.append(t)
         strides.append(_member_rows(t, C, name))
+    k_out, v_out = outs
     args = ctypes.create_string_buffer(_READ4.size)
     # An empty tensor may have no address; the library checks the rest of such a call all the same.
     _READ4.pack_into(args, 0, code, 0, row0, tokens, k_out.data_ptr() or 16, *strides[0], v_out.data_ptr() or 16,
@@ -987,11 +990,13 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, kv_
         most = int(kv_tokens)
     if not 0 <= most <= rows:
         raise PrepError(f"kv_tokens={most} outside the {rows} rows of the page table")
+    qs = _member_rows(q, C, "q")
     if out is None:
-        out = torch.empty(members, Lq, C, device=q.device, dtype=torch.bfloat16)
+        out, os_ = torch.empty(members, Lq, C, device=q.device, dtype=torch.bfloat16), (Lq * C, C)
     elif out.dtype is not torch.bfloat16 or out.get_device() != device_index or out.shape[:2] != q.shape[:2]:
         raise PrepError(f"out must be a bfloat16 [{members}, {Lq}, {C}] tensor on {pages.device}")
-    qs, os_ = _member_rows(q, C, "q"), _member_rows(out, C, "out")
+    else:
+        os_ = _member_rows(out, C, "out")
     if Lq == 0:
         return out
     args = ctypes.create_string_buffer(_ATTN4.size)
@@ -999,11 +1004,18 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, kv_
                      out.data_ptr(), *os_, lens, 0, 0, *cache)
     lib = _lib.load()
     with _on_device(device_index):
-        need = ctypes.c_int64(0)
-        _check(lib.ps_kv4_attention_workspace(args, ctypes.byref(need)))
-        if need.value:
-            if workspace is None or workspace.numel() * workspace.element_size() < need.value:
-                workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+        # The size of the partial results depends on the shape of the call alone: asked once per shape.
+        shape = (device_index, heads, Lq, most, causal_block, code, key_chunks, members, table.shape[1], pages.shape[1])
+        need = _ATTN4_NEED.get(shape)
+        if need is None:
+            asked = ctypes.c_int64(0)
+            _check(lib.ps_kv4_attention_workspace(args, ctypes.byref(asked)))
+            if len(_ATTN4_NEED) >= 4096:
+                _ATTN4_NEED.clear()
+            need = _ATTN4_NEED[shape] = asked.value
+        if need:
+            if workspace is None or workspace.numel() * workspace.element_size() < need:
+                workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
             elif workspace.get_device() != device_index or not workspace.is_contiguous():
                 raise PrepError(f"workspace must be a contiguous tensor on {pages.device}")
             struct.pack_into("=Qq", args, _ATTN4_WORKSPACE, workspace.data_ptr(),
