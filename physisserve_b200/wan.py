@@ -27,14 +27,15 @@ from typing import Sequence
 import torch
 import torch.nn.functional as F
 
-from .ops import SEQ_SINK, PrepError, Seq, _default_split, attention, flat_seq, qk_norm_rope_kv, ring_slot, rope
+from .ops import (KV4_HEAD_DIM, SEQ_SINK, PrepError, Seq, _default_split, attention, attention_kv4, flat_seq, kv4_pages,
+                  qk_norm_rope_kv, qk_norm_rope_kv4, read_kv4, ring_slot, rope)
 
 ATTENTION_SINK_CHUNKS = 1   # engine/kv_cache.py:28
 HISTORY_CHUNKS = 18         # engine/kv_cache.py:29
 FIRST_FRAMES = 3            # WanDiT.first_frames, wan.py:117
 
-__all__ = ["Attention", "RingAttention", "RingCache", "RingPositions", "prep_ring", "rope", "wan_rope_tables",
-           "window_layout"]
+__all__ = ["Attention", "Kv4Pool", "RingAttention", "RingCache", "RingCache4", "RingPositions", "prep_ring", "rope",
+           "wan_rope_tables", "window_layout"]
 
 
 def wan_rope_tables(head_dim: int, max_len: int, theta: float = 10000.0, device=None):
@@ -222,19 +223,118 @@ class RingCache:
         return (self.k[:, :n].view(shape).transpose(1, 2), self.v[:, :n].view(shape).transpose(1, 2))
 
 
+class Kv4Pool:
+    """Pages of 4-bit K/V rows (``ops.kv4_pages``) shared by the ``RingCache4`` of many cells: a cell holds
+    the pages that its window has reached and gives them back when its stream ends."""
+
+    def __init__(self, num_pages: int, heads: int, page_rows: int = 128, device=None):
+        self.pages = kv4_pages(num_pages, heads, page_rows, device)
+        self.page_rows = page_rows
+        self._free = list(range(num_pages - 1, -1, -1))
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def take(self, count: int) -> list[int]:
+        """``count`` free pages."""
+        if count > len(self._free):
+            raise PrepError(f"the pool has {len(self._free)} free pages, {count} are needed")
+        taken = self._free[len(self._free) - count:]
+        del self._free[len(self._free) - count:]
+        return taken[::-1]
+
+    def give(self, pages: Sequence[int]) -> None:
+        self._free.extend(reversed(pages))
+
+
+class RingCache4:
+    """``RingCache`` with the K/V history in 4 bits an element, in pages of a ``Kv4Pool``.
+
+    The same logical rows (sink region, then a ring of one-frame slots; window = row prefix) at 1.125 * C
+    bytes a token instead of 4 * C: what the ring would hold, rounded to e2m1 codes with an e4m3 scale for
+    16 elements (times ``k_scale`` / ``v_scale``, the tensor scales).  Pages are taken from ``pool`` as
+    the window grows and given back by ``release``.  ``sink_k`` keeps the sink's K before RoPE in the
+    activation dtype.  Heads of 128 only.
+    """
+
+    def __init__(self, *, heads: int, grid_h: int, grid_w: int, head_dim: int = KV4_HEAD_DIM,
+                 capacity: int = HISTORY_CHUNKS + 1, sink_frames: int = FIRST_FRAMES, batch: int = 1,
+                 pool: Kv4Pool | None = None, page_rows: int = 128, k_scale: float = 1.0, v_scale: float = 1.0,
+                 device=None, dtype=torch.bfloat16):
+        if head_dim != KV4_HEAD_DIM:
+            raise PrepError(f"head_dim={head_dim}: the 4-bit cache holds heads of {KV4_HEAD_DIM}")
+        self.heads, self.head_dim = heads, head_dim
+        self.grid_h, self.grid_w = grid_h, grid_w
+        self.tokens_per_frame = grid_h * grid_w
+        self.capacity, self.sink_frames, self.batch = capacity, sink_frames, batch
+        self.k_scale, self.v_scale = k_scale, v_scale
+        self.sink_rows = sink_frames * self.tokens_per_frame
+        rows = self.sink_rows + capacity * self.tokens_per_frame
+        page_rows = page_rows if pool is None else pool.page_rows
+        per_member = -(-rows // page_rows)
+        self.pool = Kv4Pool(batch * per_member, heads, page_rows, device) if pool is None else pool
+        if self.pool.pages.shape[1] != heads:
+            raise PrepError(f"the pool's pages hold {self.pool.pages.shape[1]} heads, not {heads}")
+        device = self.pool.pages.device
+        self.table = torch.full((batch, per_member), -1, dtype=torch.int32, device=device)
+        self.sink_k = torch.empty(batch, self.sink_rows, heads * head_dim, device=device, dtype=dtype)
+        self.sink_at = [None] * batch
+        self._held: list[list[int]] = [[] for _ in range(batch)]
+
+    @property
+    def pages(self) -> torch.Tensor:
+        return self.pool.pages
+
+    @property
+    def rows(self) -> int:
+        """Logical rows of a member (whole pages)."""
+        return self.table.shape[1] * self.pool.page_rows
+
+    slot = RingCache.slot
+    window_rows = RingCache.window_rows
+
+    def reserve(self, rows: Sequence[int]) -> None:
+        """Takes the pages that member b's first ``rows[b]`` rows still need."""
+        need = [-(-n // self.pool.page_rows) - len(held) for n, held in zip(rows, self._held)]
+        if sum(n for n in need if n > 0) > self.pool.free_pages:
+            raise PrepError(f"the pool has {self.pool.free_pages} free pages, {sum(n for n in need if n > 0)} are needed")
+        for b, n in enumerate(need):
+            if n > 0:
+                new, at = self.pool.take(n), len(self._held[b])
+                self.table[b, at:at + n] = torch.tensor(new, dtype=torch.int32)
+                self._held[b] += new
+
+    def release(self) -> None:
+        """Gives every page back; the cache starts over with chunk 0."""
+        for held in self._held:
+            self.pool.give(held)
+            held.clear()
+        self.table.fill_(-1)
+        self.sink_at = [None] * self.batch
+
+    def window(self, chunk: int):
+        """(K, V) windows [batch, heads, tokens, head_dim] of ``chunk``, read back in the activation dtype."""
+        n = self.window_rows(chunk)
+        k, v = read_kv4(self.pages, self.table, n, k_scale=self.k_scale, v_scale=self.v_scale, dtype=self.sink_k.dtype)
+        shape = (self.batch, n, self.heads, self.head_dim)
+        return k.view(shape).transpose(1, 2), v.view(shape).transpose(1, 2)
+
+
 def _pool_rows(caches: Sequence[RingCache]):
     """The caches of one batched call must share one storage tensor layout."""
     return caches[0].k.view(-1, caches[0].k.shape[-1])
 
 
-def prep_ring(q, k, v, q_weight, k_weight, eps, freqs_cos, freqs_sin, cache: RingCache, positions: Sequence[RingPositions],
-              *, axis_split=None, q_out=None, heads_per_thread: int = 0):
+def prep_ring(q, k, v, q_weight, k_weight, eps, freqs_cos, freqs_sin, cache: RingCache | RingCache4,
+              positions: Sequence[RingPositions], *, axis_split=None, q_out=None, heads_per_thread: int = 0):
     """One block call of a batch of streams in the ring layout.
 
     q, k, v: [batch, L, C] projection outputs of the members of ``cache`` (member b uses
     ring row block b of ``cache.k``/``cache.v``); positions[b]: its ``RingPositions``.
     Writes rotated K and V into each member's slot (sink region for chunk 0, also saving
     the pre-RoPE sink K), re-rotates relocated sinks, and returns rotated Q [batch, L, C].
+    A ``RingCache4`` takes the pages that the members' windows reach first.
     """
     B, L, C = q.shape
     if len(positions) != B or cache.batch != B:
@@ -243,8 +343,6 @@ def prep_ring(q, k, v, q_weight, k_weight, eps, freqs_cos, freqs_sin, cache: Rin
     rows = cache.rows
     if q_out is None:
         q_out = torch.empty_like(q)
-    pool_k = cache.k.view(-1, C)
-    pool_v = cache.v.view(-1, C)
     seqs, first_chunk = [], False
     for b, pos in enumerate(positions):
         if pos.frames * hw != L:
@@ -274,10 +372,14 @@ def prep_ring(q, k, v, q_weight, k_weight, eps, freqs_cos, freqs_sin, cache: Rin
              if p.chunk != 0 and cache.sink_at[b] != p.sink_position]
     seqs += [Seq(b * cache.sink_rows, cache.sink_rows, cache.grid_h, cache.grid_w, frame_offset=at,
                  ring_row=b * rows, ring_frames=cache.sink_frames, ring_slot0=0, kind=SEQ_SINK) for b, at in moved]
-    qk_norm_rope_kv(heads=cache.heads, head_dim=cache.head_dim, seqs=seqs, cos=freqs_cos, sin=freqs_sin, q=q, k=k,
-                    v=v, q_weight=q_weight, k_weight=k_weight, eps=eps, q_out=q_out, k_out=pool_k, v_out=pool_v,
-                    k_pre=k_pre, k_sink=cache.sink_k.view(-1, C) if moved else None, table_mode="axes",
-                    axis_split=axis_split, heads_per_thread=heads_per_thread)
+    call = dict(heads=cache.heads, head_dim=cache.head_dim, seqs=seqs, cos=freqs_cos, sin=freqs_sin, q=q, k=k, v=v,
+                q_weight=q_weight, k_weight=k_weight, eps=eps, q_out=q_out, k_pre=k_pre,
+                k_sink=cache.sink_k.view(-1, C) if moved else None, table_mode="axes", axis_split=axis_split)
+    if isinstance(cache, RingCache4):
+        cache.reserve([cache.window_rows(p.chunk) for p in positions])
+        qk_norm_rope_kv4(**call, pages=cache.pages, table=cache.table, k_scale=cache.k_scale, v_scale=cache.v_scale)
+    else:
+        qk_norm_rope_kv(**call, k_out=cache.k.view(-1, C), v_out=cache.v.view(-1, C), heads_per_thread=heads_per_thread)
     for b, p in enumerate(positions):
         if p.chunk == 0:
             cache.sink_at[b] = 0
@@ -289,13 +391,14 @@ def prep_ring(q, k, v, q_weight, k_weight, eps, freqs_cos, freqs_sin, cache: Rin
 class RingAttention:
     """Self-attention processor over the ring layout.
 
-    ``cache`` is a ``RingCache`` (one per stream cell, set per block call like the
+    ``cache`` is a ``RingCache`` or ``RingCache4`` (one per stream cell, set per block call like the
     reference's ``cache``) and ``rotary_emb`` is ``(freqs_cos, freqs_sin, RingPositions
     per member)``.  The attention reads the window straight from the ring storage: by default
     with the sm_100a ring attention kernel (``ops.attention``; bf16 with head_dim 128, measured
     faster than torch SDPA on the 1.3B and 14B block-call windows), with
     ``attention_kernel=False`` (or any other dtype / head size) through torch SDPA over the
-    ring views, the reference's call.
+    ring views, the reference's call.  Over a ``RingCache4`` it is ``ops.attention_kv4``, one call
+    whatever the members' window lengths, or SDPA over the window read back.
     """
 
     def __init__(self, attention_kernel: bool = True):
@@ -317,7 +420,11 @@ class RingAttention:
         if self.attention_kernel and D == 128 and q.dtype == torch.bfloat16:
             # The ring attention kernel reads each member's window rows where the prep wrote them.
             windows = [cache.window_rows(pos.chunk) for pos in positions]
-            if len(set(windows)) == 1:
+            if isinstance(cache, RingCache4):
+                rows = windows[0] if len(set(windows)) == 1 else torch.tensor(windows, dtype=torch.int32, device=q.device)
+                hidden = attention_kv4(q_rot, cache.pages, cache.table, rows, heads=heads, k_scale=cache.k_scale,
+                                       v_scale=cache.v_scale, max_kv_tokens=max(windows))
+            elif len(set(windows)) == 1:
                 hidden = attention(q_rot, cache.k, cache.v, windows[0], heads=heads)
             else:
                 hidden = torch.empty_like(q_rot)

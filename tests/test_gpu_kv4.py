@@ -552,3 +552,102 @@ def test_offsets_beyond_32_bits():
     q = torch.randn(1, 1, heads * 128, generator=g).bfloat16()
     k = torch.zeros(1, 300, heads, 128, dtype=torch.float64)
     check_attention(ops.attention_kv4(q.to(DEV), pages, table.to(DEV), 300, heads=heads), q, k, want[None], [300], heads)
+
+
+# ---------------------------------------------------------------------------------------
+# Together: the Wan ring processor over a 4-bit cache
+# ---------------------------------------------------------------------------------------
+class FakeAttn(torch.nn.Module):
+    def __init__(self, heads, C):
+        super().__init__()
+        self.heads = heads
+        self.to_q, self.to_k, self.to_v = (torch.nn.Linear(C, C, bias=False) for _ in range(3))
+        self.norm_q, self.norm_k = torch.nn.RMSNorm(C, eps=1e-6), torch.nn.RMSNorm(C, eps=1e-6)
+        self.to_out = torch.nn.ModuleList([torch.nn.Identity(), torch.nn.Identity()])
+
+
+@pytest.mark.parametrize("page_rows", [16, 128])
+def test_ring_processor_over_a_4_bit_cache(page_rows):
+    """A stream's chunks until its ring has wrapped and its sink has moved, beside the bf16 ring: the cache
+    stands for the quantised rows of the ring, and every output is the exact attention over what it holds."""
+    from physisserve_b200.wan import Kv4Pool, RingAttention, RingCache, RingCache4, wan_rope_tables, window_layout
+
+    torch.manual_seed(0)
+    heads, gh, gw, batch = 3, 3, 5, 2
+    C, hw = heads * 128, gh * gw
+    attn = FakeAttn(heads, C).to(DEV, torch.bfloat16)
+    cos, sin = wan_rope_tables(128, 64, device=DEV)
+    pool = Kv4Pool(200, heads, page_rows, device=DEV)
+    other = RingCache4(heads=heads, grid_h=gh, grid_w=gw, pool=pool)
+    other.reserve([40])                  # another cell's pages lie between
+    ring = RingCache(heads=heads, head_dim=128, grid_h=gh, grid_w=gw, batch=batch, device=DEV)
+    small = RingCache4(heads=heads, grid_h=gh, grid_w=gw, batch=batch, pool=pool, k_scale=0.9, v_scale=0.5)
+    kernel, plain = RingAttention(), RingAttention()
+    sdpa = RingAttention(attention_kernel=False)
+    ops.kv4_counters()
+    for chunk in range(24):
+        pos = [window_layout(chunk)] * batch
+        x = torch.randn(batch, pos[0].frames * hw, C, device=DEV).bfloat16()
+        kernel.cache, plain.cache, sdpa.cache = small, ring, small
+        with torch.no_grad():
+            got = kernel(attn, x, rotary_emb=(cos, sin, pos))
+            plain(attn, x, rotary_emb=(cos, sin, pos))
+            q = attn.to_q(x)
+        n = small.window_rows(chunk)
+        k4, v4 = ops.read_kv4(small.pages, small.table, n, k_scale=0.9, v_scale=0.5, dtype=torch.float32)
+        for have, held, which, scale in ((k4, ring.k, 0, 0.9), (v4, ring.v, 1, 0.5)):
+            rows = held[:, :n].cpu().view(batch * n, heads, 128)
+            want = kv4.dequantise(*kv4.quantise(rows, scale), scale).view(batch, n, C)
+            # K's sum of squares has another order in the ring: a bf16 rounding in 10^4 may differ.
+            differ = (have.cpu().double() - want).abs() > 2 ** -20 * want.abs()
+            assert float(differ.float().mean()) <= (1e-3 if which == 0 else 0.0)
+        q_rot = _rotated_q(attn, q, cos, sin, pos[0], heads, gh, gw)
+        check_attention(got, q_rot, k4.cpu().double().view(batch, n, heads, 128), v4.cpu().double().view(batch, n, heads, 128),
+                        [n] * batch, heads)
+        if chunk in (0, 5, 23):          # SDPA over the window read back: the same to bf16 probabilities
+            with torch.no_grad():
+                again = sdpa(attn, x, rotary_emb=(cos, sin, pos))
+            assert float((again.float() - got.float()).abs().max()) <= 2 ** -5 * float(got.float().abs().max())
+    assert ops.kv4_counters() == (0, 0, 0)
+    used = pool.free_pages
+    small.release()
+    assert pool.free_pages > used
+
+
+def _rotated_q(attn, q, cos, sin, pos, heads, gh, gw):
+    """Q as the prep kernel leaves it, from the library itself (tested bit for bit above)."""
+    B, L, C = q.shape
+    out = torch.empty_like(q)
+    seqs = [ops.Seq(b * L, L, gh, gw, pos.frame_offset) for b in range(B)]
+    pages = ops.kv4_pages(1, heads, 16, DEV)
+    ops.qk_norm_rope_kv4(heads=heads, seqs=seqs, cos=cos, sin=sin, q=q, q_weight=attn.norm_q.weight.detach(), q_out=out,
+                         pages=pages, table=torch.zeros(1, 1, dtype=torch.int32, device=DEV))
+    return out.cpu()
+
+
+def test_ring_processor_members_at_different_chunks():
+    """Members whose windows differ: one call with the lengths on the device."""
+    from physisserve_b200.wan import RingAttention, RingCache4, wan_rope_tables, window_layout
+
+    torch.manual_seed(1)
+    heads, gh, gw = 2, 2, 4
+    C, hw = heads * 128, gh * gw
+    attn = FakeAttn(heads, C).to(DEV, torch.bfloat16)
+    cos, sin = wan_rope_tables(128, 64, device=DEV)
+    cache = RingCache4(heads=heads, grid_h=gh, grid_w=gw, batch=2, page_rows=16, device=DEV)
+    proc = RingAttention()
+    proc.cache = cache
+    with torch.no_grad():
+        proc(attn, torch.randn(2, 3 * hw, C, device=DEV).bfloat16(), rotary_emb=(cos, sin, [window_layout(0)] * 2))
+        for chunks in ((1, 1), (2, 1), (3, 2), (3, 4)):
+            pos = [window_layout(c) for c in chunks]
+            x = torch.randn(2, hw, C, device=DEV).bfloat16()
+            got = proc(attn, x, rotary_emb=(cos, sin, pos))
+            lens = [cache.window_rows(c) for c in chunks]
+            n = max(lens)
+            k, v = ops.read_kv4(cache.pages, cache.table, n, dtype=torch.float32)
+            q = attn.to_q(x)
+            q_rot = torch.cat([_rotated_q(attn, q[b:b + 1], cos, sin, pos[b], heads, gh, gw) for b in range(2)])
+            check_attention(got, q_rot, k.cpu().double().view(2, n, heads, 128), v.cpu().double().view(2, n, heads, 128), lens,
+                            heads)
+    ops.kv4_counters()

@@ -230,3 +230,37 @@ def test_wrappers_refuse_cpu_tensors_and_bad_pools():
         ops.read_kv4(pages.int(), table, 4)
     with pytest.raises(ops.PrepError, match="bytes a head"):
         ops.read_kv4(pages[..., :100].contiguous(), table, 4)
+
+
+# ---------------------------------------------------------------------------------------
+# The pool of the Wan ring caches
+# ---------------------------------------------------------------------------------------
+def test_pool_hands_out_every_page_once_and_takes_them_back():
+    from physisserve_b200.wan import Kv4Pool, RingCache4
+
+    pool = Kv4Pool(7, 2, page_rows=16)
+    a, b = (RingCache4(heads=2, grid_h=2, grid_w=5, capacity=4, sink_frames=2, batch=n, pool=pool) for n in (1, 2))
+    assert a.rows == 64 and b.rows == 64 and a.window_rows(0) == 20 and a.window_rows(9) == 60
+    a.reserve([20])
+    b.reserve([16, 33])
+    assert pool.free_pages == 1
+    held = [int(p) for cache in (a, b) for p in cache.table.flatten() if p >= 0]
+    assert len(held) == len(set(held)) == 6
+    a.reserve([20])                      # nothing more is needed
+    assert pool.free_pages == 1
+    with pytest.raises(ops.PrepError, match="free pages"):
+        b.reserve([64, 64])
+    assert pool.free_pages == 1          # a refused reservation takes nothing
+    b.release()
+    assert pool.free_pages == 5 and bool((b.table == -1).all())
+    a.reserve([60])
+    assert pool.free_pages == 3 and [int(p) for p in a.table[0, :2]] == held[:2]
+
+
+def test_ring_cache_refuses_other_heads():
+    from physisserve_b200.wan import Kv4Pool, RingCache4
+
+    with pytest.raises(ops.PrepError, match="128"):
+        RingCache4(heads=2, head_dim=64, grid_h=2, grid_w=5)
+    with pytest.raises(ops.PrepError, match="heads"):
+        RingCache4(heads=2, grid_h=2, grid_w=5, pool=Kv4Pool(4, 3))
