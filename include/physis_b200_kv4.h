@@ -61,7 +61,9 @@ typedef struct ps_kv4_cache {
 /* Arguments of ps_qk_norm_rope_kv4.  As ps_qk_prep_args, with the K and V rows
  * going to the cache: ring_row, ring_frames and ring_slot0 of a sequence name
  * logical rows of the cache (a member's rows start at member * table_pages *
- * page_rows; a sequence's ring lies within one member's rows). */
+ * page_rows).  No two tokens of a launch may go to the same row of the same page,
+ * by equal ring rows or by a page that stands in the table twice: which of them
+ * the row then holds is not defined. */
 typedef struct ps_kv4_prep_args {
   int32_t dtype;      /* ps_dtype of q, k, v, q_out, k_pre and k_sink */
   int32_t heads;      /* query heads */
@@ -71,7 +73,8 @@ typedef struct ps_kv4_prep_args {
   int32_t n_seqs;     /* 1..PS_MAX_SEQS */
   float eps;          /* RMSNorm epsilon */
   int32_t weight_f32; /* 0: weights are of dtype; 1: fp32 */
-  int32_t launch;     /* ps_launch */
+  int32_t launch;     /* ps_launch; PS_LAUNCH_PDL_EARLY_INPUTS reads the page table before
+                       * the wait too: no kernel still running may write it */
   int32_t reserved;   /* 0 */
 
   int64_t in_rows;                    /* rows of q, k, v, q_out, k_pre */
@@ -125,7 +128,7 @@ typedef struct ps_kv4_attn_args {
   int32_t causal_block; /* 0: no mask */
   float scale;          /* softmax scale; <= 0 selects 1/sqrt(128) */
   int32_t kernel;       /* ps_kv4_kernel */
-  int32_t key_chunks;   /* key chunks per unit of work, 1..64; 0 = automatic */
+  int32_t key_chunks;   /* rows kernel: key chunks per block of rows, 1..64; 0 = automatic */
   int32_t reserved;     /* 0 */
   const void* q;  int64_t q_member_stride;   int64_t q_row_stride;   /* bf16 */
   void* out;      int64_t out_member_stride; int64_t out_row_stride; /* bf16 */
@@ -155,6 +158,7 @@ PS_API int32_t ps_kv4_read_validate(const ps_kv4_read_args* args);
  * are rounded to fp16 for P V; the output is rounded once to bf16. */
 PS_API int32_t ps_attention_kv4(const ps_kv4_attn_args* args, void* stream);
 PS_API int32_t ps_kv4_attention_validate(const ps_kv4_attn_args* args);
+/* Bytes of scratch that ps_attention_kv4 needs for these arguments on the current device. */
 PS_API int32_t ps_kv4_attention_workspace(const ps_kv4_attn_args* args, int64_t* bytes);
 
 /* Counts on the current device since the last reset: counts[0] accesses to pages

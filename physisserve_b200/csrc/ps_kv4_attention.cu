@@ -1365,7 +1365,7 @@ static int build_attn(const ps_kv4_attn_args* a, APlan* plan, bool host_only) {
   if (rows > (1 << 30)) return fail(PS_ERR_UNSUPPORTED, "%lld query rows of a K/V head", (long long)rows);
   p.rows = static_cast<int32_t>(rows);
   const int tiles = (a->kv_tokens + kTileKeys - 1) / kTileKeys;
-  const int sms = host_only ? 148 : sm_count();
+  const int sms = sm_count();
   plan->kernel = a->kernel;
   if (plan->kernel == PS_KV4_AUTO) {
     // The rows kernel passes over the keys once per 8 query rows, 0.62 us a 128-key tile on an SM; the tiles
@@ -1381,10 +1381,12 @@ static int build_attn(const ps_kv4_attn_args* a, APlan* plan, bool host_only) {
   const bool tiles_kernel = plan->kernel == PS_KV4_TILES;
   plan->block_rows = tiles_kernel ? kUnitRows : kBlockRows;
   p.row_blocks = (p.rows + plan->block_rows - 1) / plan->block_rows;
+  if (p.row_blocks > 0 && a->cache.members * hk > (1 << 26) / p.row_blocks)
+    return fail(PS_ERR_UNSUPPORTED, "%lld members of %d K/V heads and %d row blocks", (long long)a->cache.members, hk,
+                p.row_blocks);
   p.units = a->cache.members * hk * p.row_blocks;
   const double scale = a->scale > 0.f ? a->scale : 1.0 / sqrt(static_cast<double>(kKv4D));
   p.scale_log2 = static_cast<float>(scale * a->cache.k_scale * 1.4426950408889634);
-  if (p.units > (1 << 26)) return fail(PS_ERR_UNSUPPORTED, "%lld units of work", (long long)p.units);
   int64_t slots;
   if (tiles_kernel) {
     p.chunks = 1;

@@ -725,6 +725,8 @@ def _kv4_cache(pages: torch.Tensor, table: torch.Tensor, k_scale: float, v_scale
     device_index = pages.get_device()
     if table.get_device() != device_index:
         raise PrepError(f"tensors on different devices: {pages.device} and {table.device}")
+    if not (1e-20 <= k_scale <= 1e20 and 1e-20 <= v_scale <= 1e20):
+        raise PrepError(f"tensor scales {k_scale} and {v_scale} outside [1e-20, 1e20]")
     members, table_pages = table.shape
     return device_index, members, page_rows, (pages.data_ptr(), table.data_ptr(), pages.shape[0], members, table_pages,
                                               pages.shape[1], page_rows, k_scale, v_scale)
@@ -851,7 +853,8 @@ def qk_norm_rope_kv4(**kwargs) -> None:
     float32, any row stride), ``q_weight``/``k_weight``, ``eps``, ``q_out``, ``k_pre``, ``k_sink`` (pre-RoPE
     K rows of ``SEQ_SINK`` sequences), ``k_scale``/``v_scale`` (tensor scales of the cache: an element is
     code * block scale * tensor scale, at most 2688 tensor scales), ``table_mode``, ``axis_split`` and
-    ``launch`` as in ``qk_norm_rope_kv``.  NaN is stored as zero and infinities saturate; both, and
+    ``launch`` as in ``qk_norm_rope_kv`` ("pdl_early_inputs" reads the page table early too).  No two
+    tokens of a call may go to the same row of the same page.  NaN is stored as zero and infinities saturate; both, and
     page numbers outside the pool (their rows are skipped), are counted in ``kv4_counters``.
     """
     device_index, parts, _ = _prepare4(**kwargs)
@@ -958,8 +961,8 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, kv_
     ``causal_block`` c > 0 lets query row t see the rows below ``min(n, n - Lq + (t // c + 1) * c)`` of
     a member's n: 1 is the causal mask, the tokens of a frame let a frame see itself and the frames
     before it.  A row that sees nothing gets zeros.  Returns ``out`` [B, Lq, heads*128] (allocated if
-    not given).  ``kernel`` ("auto", "rows", "tiles") and ``key_chunks`` override the kernel and the work
-    split; ``workspace`` is a byte tensor for the partial results of key chunks (allocated if None or
+    not given).  ``kernel`` ("auto", "rows", "tiles") and ``key_chunks`` override the kernel and the rows
+    kernel's work split; ``workspace`` is a byte tensor for the partial results of key chunks (allocated if None or
     too small).  ``check_timeouts=True`` synchronises and raises ``PrepError`` if a bounded wait ran out.
     """
     device_index, members, page_rows, cache = _kv4_cache(pages, table, k_scale, v_scale)

@@ -231,6 +231,7 @@ class Kv4Pool:
         self.pages = kv4_pages(num_pages, heads, page_rows, device)
         self.page_rows = page_rows
         self._free = list(range(num_pages - 1, -1, -1))
+        self._taken: set[int] = set()
 
     @property
     def free_pages(self) -> int:
@@ -242,9 +243,16 @@ class Kv4Pool:
             raise PrepError(f"the pool has {len(self._free)} free pages, {count} are needed")
         taken = self._free[len(self._free) - count:]
         del self._free[len(self._free) - count:]
+        self._taken.update(taken)
         return taken[::-1]
 
     def give(self, pages: Sequence[int]) -> None:
+        """Takes pages back.  Work on them that is still running on another stream than the one their
+        next holder uses must be waited for first."""
+        given = set(pages)
+        if len(given) != len(pages) or not given <= self._taken:
+            raise PrepError(f"pages {list(pages)} are not all held by someone, each once")
+        self._taken -= given
         self._free.extend(reversed(pages))
 
 
@@ -295,14 +303,19 @@ class RingCache4:
     window_rows = RingCache.window_rows
 
     def reserve(self, rows: Sequence[int]) -> None:
-        """Takes the pages that member b's first ``rows[b]`` rows still need."""
+        """Takes the pages that member b's first ``rows[b]`` rows still need (outside of a captured graph: the
+        new table entries are copied from the host; a graph's windows are reserved ahead of it)."""
         need = [-(-n // self.pool.page_rows) - len(held) for n, held in zip(rows, self._held)]
         if sum(n for n in need if n > 0) > self.pool.free_pages:
             raise PrepError(f"the pool has {self.pool.free_pages} free pages, {sum(n for n in need if n > 0)} are needed")
         for b, n in enumerate(need):
             if n > 0:
                 new, at = self.pool.take(n), len(self._held[b])
-                self.table[b, at:at + n] = torch.tensor(new, dtype=torch.int32)
+                try:
+                    self.table[b, at:at + n] = torch.tensor(new, dtype=torch.int32)
+                except RuntimeError:  # a copy from the host fails in a captured graph
+                    self.pool.give(new)
+                    raise
                 self._held[b] += new
 
     def release(self) -> None:
@@ -398,7 +411,8 @@ class RingAttention:
     faster than torch SDPA on the 1.3B and 14B block-call windows), with
     ``attention_kernel=False`` (or any other dtype / head size) through torch SDPA over the
     ring views, the reference's call.  Over a ``RingCache4`` it is ``ops.attention_kv4``, one call
-    whatever the members' window lengths, or SDPA over the window read back.
+    whatever the members' window lengths (unlike ones are copied from the host: not in a captured
+    graph), or SDPA over the window read back.
     """
 
     def __init__(self, attention_kernel: bool = True):

@@ -256,6 +256,37 @@ def test_append_bad_pages_are_skipped_and_counted():
     assert ops.kv4_counters().bad_pages > 0
 
 
+@pytest.mark.parametrize("launch", ["stream", "pdl", "pdl_early_inputs"])
+def test_append_launch_modes_store_the_same(launch):
+    """A chain of appends of independent inputs, each read back by the next kernel on the stream."""
+    cases = [append_case(2, 5, 7, 2, 12, 4, 32, torch.bfloat16, 2, seed=s) for s in range(4)]
+    torch.cuda.synchronize()             # the inputs are there before the first launch
+    back = []
+    for kwargs, _, _, _ in cases:
+        ops.qk_norm_rope_kv4(**kwargs, launch=launch)
+        back.append(ops.read_kv4(kwargs["pages"], kwargs["table"], 70, v_scale=0.375))
+    for (kwargs, want, q_ref, _), (k, v) in zip(cases, back):
+        assert torch.equal(kwargs["pages"].cpu(), want)
+        check_q(kwargs["q_out"], q_ref, torch.bfloat16)
+        flat = torch.arange(70)
+        for which, x, scale in ((0, k, 1.0), (1, v, 0.375)):
+            for b in range(2):
+                ref = kv4.load(want, kwargs["table"].cpu()[b:b + 1], flat, which, scale)
+                assert bool(((x[b].cpu().double().view(ref.shape) - ref).abs() <= 2 ** -8 * ref.abs()).all())
+
+
+def test_append_on_another_stream_than_the_current_one_before():
+    kwargs, want, q_ref, _ = append_case(2, 3, 5, 1, 4, 4, 16, torch.bfloat16, 2, seed=3)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.qk_norm_rope_kv4(**kwargs)
+        k, _ = ops.read_kv4(kwargs["pages"], kwargs["table"], 30)
+    side.synchronize()
+    assert torch.equal(kwargs["pages"].cpu(), want) and bool(k.any())
+    check_q(kwargs["q_out"], q_ref, torch.bfloat16)
+
+
 def test_append_plan_swaps_tensors():
     case = (2, 3, 5, 1, 4, 4, 16, torch.bfloat16, 2)
     kwargs, _, _, _ = append_case(*case, seed=1)
@@ -503,6 +534,73 @@ def test_two_graphs_and_an_eager_call_do_not_share_partial_results():
         check_attention(out, q, k, v, [3000], 2)
 
 
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
+@pytest.mark.parametrize("Lq", [1, 200])
+def test_members_that_share_pages(Lq, kernel):
+    """A page may stand in the table more than once: a prefix that two members share, a page twice in one."""
+    pages, table, k, v = fill(1, 320, 2, 64, 23, extra_pages=0)
+    first = table[0]
+    shared = torch.stack([first, torch.stack([first[0], first[1], first[1], first[4], first[0]])])
+    at = torch.cat([torch.arange(64) + 64 * i for i in (0, 1, 1, 4, 0)])
+    k, v = torch.stack([k[0], k[0, at]]), torch.stack([v[0], v[0, at]])
+    q = torch.randn(2, Lq, 2 * 128, generator=gen(24)).bfloat16()
+    got = ops.attention_kv4(q.to(DEV), pages.to(DEV), shared.to(DEV), 320, heads=2, kernel=kernel)
+    check_attention(got, q, k, v, [320] * 2, 2)
+
+
+def test_a_captured_decoding_step_appends_and_attends():
+    """One graph of append and attention, replayed for token after token: the lengths, the page table and the
+    inputs change in place between replays; the same steps without a graph give the same bytes."""
+    heads, hk, members, page_rows, steps = 8, 2, 2, 16, 20
+    n_pages, table = make_table(members, 2, 3, 5)
+    cos, sin = (t.to(DEV) for t in wan_prep.rope_tables(128, 256))
+    x = torch.randn(steps, members, (heads + 2 * hk) * 128, generator=gen(6)).bfloat16().to(DEV)
+
+    def run(captured):
+        pages = ops.kv4_pages(n_pages, hk, page_rows, DEV)
+        dt, lens = table.to(DEV), torch.zeros(members, dtype=torch.int32, device=DEV)
+        row = torch.zeros(members, heads * 128 + 2 * hk * 128, dtype=torch.bfloat16, device=DEV)
+        q, k, v = row.split((heads * 128, hk * 128, hk * 128), 1)
+        # The ring of a step is one row, the first of the member's table: the table entry of that row moves on.
+        step_table, q_out = dt.clone(), torch.empty(members, heads * 128, dtype=torch.bfloat16, device=DEV)
+        plans = [ops.Prep4Plan(heads=heads, seqs=[ops.Seq(b, 1, 1, 1, 0, 0, b * 2 * page_rows + r, 1, 0)
+                                                  for b in range(members)], cos=cos, sin=sin, q=q, k=k, v=v,
+                               q_out=q_out, pages=pages, table=step_table) for r in range(page_rows)]
+        out = torch.empty(members, 1, heads * 128, dtype=torch.bfloat16, device=DEV)
+
+        def step(r):
+            plans[r].launch()
+            ops.attention_kv4(q_out.view(members, 1, -1), pages, dt, lens, heads=heads, out=out)
+
+        graphs = {}
+        if captured:
+            step(0)
+            pages.zero_()
+            torch.cuda.synchronize()
+            for r in range(page_rows):
+                graphs[r] = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graphs[r]):
+                    step(r)
+        outs = []
+        for t in range(steps):
+            row.copy_(x[t])
+            lens.fill_(t + 1)
+            step_table[:, 0] = dt[:, t // page_rows]
+            graphs[t % page_rows].replay() if captured else step(t % page_rows)
+            outs.append(out.clone())
+        return torch.stack(outs), pages
+
+    outs, pages = run(False)
+    outs2, pages2 = run(True)
+    assert torch.equal(outs, outs2) and torch.equal(pages, pages2)
+    flat = torch.arange(members)[:, None] * 2 * page_rows + torch.arange(steps)
+    k, v = (kv4.load(pages.cpu(), table, flat.flatten(), w, 1.0).view(members, steps, hk, 128) for w in (0, 1))
+    c, s = (t[:1, None].cpu() for t in (cos, sin))
+    for t in (0, 15, 16, 19):
+        q = wan_prep.rope(x[t, :, :heads * 128].cpu().view(1, members, heads, 128), c[None], s[None])[0].flatten(1)
+        check_attention(outs[t], q.view(members, 1, -1), k[:, :t + 1], v[:, :t + 1], [t + 1] * members, heads)
+
+
 def test_results_do_not_depend_on_the_run():
     pages, table, _, _ = fill(2, 2000, 2, 64, 16)
     for Lq in (1, 300):
@@ -529,6 +627,12 @@ def test_attention_refusals():
         ops.attention_kv4(q, dp, dt, 50, heads=4, out=torch.empty(2, 4, 512, dtype=torch.bfloat16, device=DEV))
     with pytest.raises(ops.PrepError, match="kernel"):
         ops.attention_kv4(q, dp, dt, 50, heads=4, kernel="fast")
+    for bad in (0.0, -1.0, 1e300, float("nan")):
+        with pytest.raises(ops.PrepError, match="tensor scales"):
+            ops.attention_kv4(q, dp, dt, 50, heads=4, k_scale=bad)
+    with pytest.raises(ops.PrepError, match="workspace"):
+        ops.attention_kv4(q, dp, dt, 50, heads=4, kernel="tiles",
+                          workspace=torch.empty(1 << 22, dtype=torch.uint8, device=DEV)[1:])
     assert ops.attention_kv4(q[:, :0], dp, dt, 50, heads=4).shape == (2, 0, 512)
 
 

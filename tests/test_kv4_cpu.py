@@ -198,6 +198,15 @@ def test_attention_refusals(lib, change, status):
     refused(lib, "ps_kv4_attention_validate", attn(**change), status)
 
 
+def test_attention_refuses_more_work_than_a_grid_holds(lib):
+    big = attn(q_tokens=1 << 29)
+    big.cache.members = 1 << 24
+    big.cache.kv_heads, big.heads = 1024, 1024
+    big.q_row_stride = big.out_row_stride = 1024 * 128
+    big.q_member_stride = big.out_member_stride = (1 << 29) * 1024 * 128
+    assert lib.ps_kv4_attention_validate(ctypes.byref(big)) == _lib.ERR_UNSUPPORTED
+
+
 def test_attention_without_its_workspace_is_refused_before_any_launch(lib):
     """ps_attention_kv4 itself checks the workspace on the host; the size is what the query reports."""
     big = cache(table_pages=1000, num_pages=5000)
@@ -255,6 +264,20 @@ def test_pool_hands_out_every_page_once_and_takes_them_back():
     assert pool.free_pages == 5 and bool((b.table == -1).all())
     a.reserve([60])
     assert pool.free_pages == 3 and [int(p) for p in a.table[0, :2]] == held[:2]
+
+
+def test_pool_takes_back_only_what_it_gave():
+    from physisserve_b200.wan import Kv4Pool
+
+    pool = Kv4Pool(4, 1, page_rows=16)
+    held = pool.take(2)
+    for bad in ([held[0], held[0]], [3 if 3 not in held else 0], [7]):
+        with pytest.raises(ops.PrepError, match="held"):
+            pool.give(bad)
+    pool.give(held)
+    with pytest.raises(ops.PrepError, match="held"):
+        pool.give(held[:1])
+    assert sorted(pool.take(4)) == [0, 1, 2, 3]
 
 
 def test_ring_cache_refuses_other_heads():
