@@ -29,15 +29,16 @@ struct AParams {
   int32_t Lq, kv_max, causal_block, group;
   int32_t rows;          // query rows of a K/V head: Lq * group
   int32_t row_blocks;    // blocks of query rows per K/V head
-  int32_t chunks;        // rows kernel: key chunks per unit
+  int32_t chunks;        // rows kernel: key chunks per unit; 0: by the members' lengths (plan_split)
   int32_t grid;          // tiles kernel: persistent CTAs
   int32_t min_steps;     // tiles kernel: fewest steps of a CTA
   int64_t units;         // members * kv_heads * row_blocks
   float scale_log2;      // softmax scale * k_scale * log2(e)
   float* ws_o;           // partial results: [slots][rows of a block][128] unnormalised sums,
   float2* ws_ml;         // [slots][rows of a block] (reference in log2 units, sum); slots are
-                         // [units][chunks] (rows kernel) or [grid][2] (tiles kernel)
-  int4* ws_units;        // tiles kernel: [units] (first CTA, last CTA, the first CTA's slot, 0)
+                         // [CTAs] (rows kernel) or [grid][2] (tiles kernel)
+  int4* ws_units;        // tiles kernel: [units] (first CTA, last CTA, the first CTA's slot, 0);
+                         // rows kernel without fixed chunks: [members] (Split::before, Split::chunks)
 };
 
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int* abort_flag, bool count = true) {
@@ -160,12 +161,77 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
       : "r"(taddr));
 }
 
+// Which keys a CTA of the rows kernel takes.  The chunks of all members stand in a row, `before` of them ahead of
+// this member's; each is kv_heads * row_blocks CTAs.  chunks == 0: the CTA has no work.
+struct Split {
+  int member, before, chunks;
+};
+
 struct RowsShared {
   alignas(128) unsigned char stage[kStages][kTileBytes];
   alignas(8) unsigned long long full[kStages], empty[kStages];
   uint32_t bad[kStages];  // bit s: segment (page) s of the tile is not in the pool
+  int lim[kBlockRows];    // keys that each query row sees
+  Split split;
   int abort;
 };
+
+// Members of unlike length get chunks of like length: the fewest tiles a chunk, out of four sizes between the mean
+// and one that always fits, with which all chunks find a CTA of the grid.  By one warp.
+constexpr int kMinChunkTiles = 2;  // fewest tiles of a chunk (12 heads over 1 716 keys: 10.1 us, with four 11.8)
+__device__ __noinline__ Split plan_split(const AParams& p, int lane) {
+  const int per = p.cache.kv_heads * p.row_blocks, members = static_cast<int>(p.units / per);
+  const int room = static_cast<int>(gridDim.x) / per, at = static_cast<int>(blockIdx.x) / per;
+  auto tiles_of = [&](int b) { return b < members ? (member_len(p, b) + kTileKeys - 1) / kTileKeys : 0; };
+  int64_t sum = 0;
+  int top = 0;
+  for (int b = lane; b < members; b += 32) {
+    const int t = tiles_of(b);
+    sum += t;
+    top = max(top, t);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+  }
+  const int low = max(max(kMinChunkTiles, (top + kMaxChunks - 1) / kMaxChunks), static_cast<int>((sum + room - 1) / room));
+  // Sum of ceil(t / size) <= sum / size + members: with `high` everything fits.
+  const int64_t fits = room > members ? (sum + room - members - 1) / (room - members) : top;
+  const int high = max(low, static_cast<int>(min(fits, static_cast<int64_t>(top))));
+  int size[4], need[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    size[i] = low + static_cast<int>(static_cast<int64_t>(high - low) * i / 4);
+    need[i] = 0;
+  }
+  for (int b = lane; b < members; b += 32) {
+    const int t = tiles_of(b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) need[i] += max(1, (t + size[i] - 1) / size[i]);
+  }
+  int chosen = high;
+#pragma unroll
+  for (int i = 3; i >= 0; --i)
+    if (static_cast<int>(__reduce_add_sync(0xffffffffu, need[i])) <= room) chosen = size[i];
+  int before = 0;
+  for (int b0 = 0; b0 < members; b0 += 32) {
+    const int own = b0 + lane < members ? max(1, (tiles_of(b0 + lane) + chosen - 1) / chosen) : 0;
+    int upto = own;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += x;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, at < before + upto);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      return Split{b0 + l, before + __shfl_sync(0xffffffffu, upto - own, l), __shfl_sync(0xffffffffu, own, l)};
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return Split{0, 0, 0};
+}
 
 __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_constant__ AParams p) {
   constexpr int R = kBlockRows;
@@ -180,28 +246,37 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
       bar_init(saddr(&sh.empty[s]), kRowWarps);
     }
     sh.abort = 0;
+    if (p.chunks) {
+      const int member = static_cast<int>(blockIdx.x / (static_cast<int64_t>(p.cache.kv_heads) * p.row_blocks * p.chunks));
+      sh.split = Split{member, member * p.chunks, p.chunks};
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (p.chunks == 0 && warp == 1) {
+    pdl_wait();  // the lengths may come from the kernel before
+    const Split split = plan_split(p, lane);
+    if (lane == 0) sh.split = split;
   }
   __syncthreads();
 
-  // CTA -> (unit, chunk): the row blocks of a (member, head, chunk) are neighbours, so that the keys
-  // they share come from L2.
-  int64_t at = blockIdx.x;
-  const int rb = static_cast<int>(at % p.row_blocks);
+  // The row blocks of a (member, head, chunk) are neighbours, so that the keys they share come from L2.
+  const Split split = sh.split;
+  if (split.chunks == 0) return;
+  const int per = p.cache.kv_heads * p.row_blocks;
+  int at = static_cast<int>(blockIdx.x - static_cast<int64_t>(split.before) * per);
+  const int rb = at % p.row_blocks;
   at /= p.row_blocks;
-  const int chunk = static_cast<int>(at % p.chunks);
-  at /= p.chunks;
-  const int b = static_cast<int>(at / p.cache.kv_heads), h = static_cast<int>(at % p.cache.kv_heads);
-  const int64_t unit = at * p.row_blocks + rb;
-
+  const int chunk = at % split.chunks, h = at / split.chunks, b = split.member;
+  if (p.chunks == 0 && at == 0 && rb == 0 && threadIdx.x == 0)
+    p.ws_units[b] = make_int4(split.before, split.chunks, 0, 0);
   pdl_wait();
   const int n = member_len(p, b);
   const int row0 = rb * R, row_end = min(row0 + R, p.rows);
   const int lim_low = token_limit(p, n, row0 / p.group);               // fewest keys of any row of the block
   const int lim_top = token_limit(p, n, (row_end - 1) / p.group);      // most keys
   const int tiles = (lim_top + kTileKeys - 1) / kTileKeys;
-  const int j0 = static_cast<int>(static_cast<int64_t>(chunk) * tiles / p.chunks);
-  const int j1 = static_cast<int>(static_cast<int64_t>(chunk + 1) * tiles / p.chunks);
+  const int j0 = static_cast<int>(static_cast<int64_t>(chunk) * tiles / split.chunks);
+  const int j1 = static_cast<int>(static_cast<int64_t>(chunk + 1) * tiles / split.chunks);
   const int shift = p.cache.shift, page_rows = 1 << shift;
   const int segs = kTileKeys >> shift;  // pages per tile
   const uint32_t seg_bytes = static_cast<uint32_t>(p.cache.head_bytes);
@@ -209,6 +284,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
   if (warp == kRowWarps) {
     // ------------------------------- producer -------------------------------
     int t = 0;
+    if (lane < R) sh.lim[lane] = token_limit(p, n, min(row0 + lane, p.rows - 1) / p.group);
     // Lane i: table entry of the tile's page i, a tile ahead (unconditional loads, so that nothing waits for
     // them before they are used).
     auto seen = [&](int j) { return lane < segs && j * kTileKeys + (lane << shift) < lim_top; };
@@ -294,10 +370,9 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
     const int v_base = page_rows * kKv4Row;
     const int v_codes = v_base + g * 8, v_scale = v_base + page_rows * 64 + g;
 
-    int t = 0;
-    for (int j = j0; j < j1; ++j, ++t) {
-      const int s = t % kStages;
-      if (!warp_wait(saddr(&sh.full[s]), (t / kStages) & 1, abort_flag, lane)) break;
+    int s = 0, phase = 0;
+    for (int j = j0; j < j1; ++j) {
+      if (!warp_wait(saddr(&sh.full[s]), phase, abort_flag, lane)) break;
       const uint32_t bad = *reinterpret_cast<volatile uint32_t*>(&sh.bad[s]);
       const bool masked = (j + 1) * kTileKeys > lim_low || bad != 0;
       // This warp's 32 keys, two groups of 16 side by side: a group's products are chains of dependent MMAs,
@@ -342,7 +417,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
       if (masked) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int lim = token_limit(p, n, min(row0 + 2 * c + e, p.rows - 1) / p.group) - j * kTileKeys;
+          const int lim = *const_cast<volatile int*>(&sh.lim[2 * c + e]) - j * kTileKeys;
 #pragma unroll
           for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -407,6 +482,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
           sc[i] = base[v_scale + r * 8];
         }
         if (masked) {  // rows that no query row sees and rows of a missing page hold anything: 0 * code = 0
+        const int lim_top = *const_cast<volatile int*>(&sh.lim[R - 1]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int in_tile = key + (i & 1 ? v1 : v0) + (i >> 1) * 8;
@@ -433,6 +509,10 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
       }
       __syncwarp();
       if (lane == 0) bar_arrive(saddr(&sh.empty[s]));
+      if (++s == kStages) {
+        s = 0;
+        phase ^= 1;
+      }
     }
     // The rows' sums over the lanes that share them.
 #pragma unroll
@@ -460,7 +540,12 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
   }
   __syncthreads();
   if (warp == kRowWarps) return;
-  for (int r = warp; r < row_end - row0; r += kRowWarps) {
+  // Where the rows go: decoded once more, so that nothing of it stays in registers over the keys.
+  const volatile Split& own = sh.split;
+  const int chunks = own.chunks, member = own.member;
+  const int in_member = static_cast<int>(blockIdx.x - static_cast<int64_t>(own.before) * p.cache.kv_heads * p.row_blocks);
+  const int first_row = in_member % p.row_blocks * R, head = in_member / p.row_blocks / chunks;
+  for (int r = warp; r < min(R, p.rows - first_row); r += kRowWarps) {
     float top = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, stat[w * R + r].x);
@@ -478,15 +563,15 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
       x.z += f * y.z;
       x.w += f * y.w;
     }
-    if (p.chunks > 1) {
-      const int64_t slot = (unit * p.chunks + chunk) * R + r;
+    if (chunks > 1) {
+      const int64_t slot = static_cast<int64_t>(blockIdx.x) * R + r;
       *reinterpret_cast<float4*>(p.ws_o + slot * kKv4D + 4 * lane) = x;
       if (lane == 0) p.ws_ml[slot] = make_float2(top, sum);
     } else {
       const float inv = sum == 0.f ? 0.f : p.cache.v_scale / sum;
-      const int row = row0 + r, t = row / p.group;
+      const int row = first_row + r, t = row / p.group;
       __nv_bfloat16* dst =
-          p.out + b * p.out_member + t * p.out_row + (h * p.group + (row - t * p.group)) * kKv4D + 4 * lane;
+          p.out + member * p.out_member + t * p.out_row + (head * p.group + (row - t * p.group)) * kKv4D + 4 * lane;
       *reinterpret_cast<uint2*>(dst) = make_uint2(Pairs16<__nv_bfloat16>::pack_pair(x.x * inv, x.y * inv),
                                                   Pairs16<__nv_bfloat16>::pack_pair(x.z * inv, x.w * inv));
     }
@@ -494,22 +579,32 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
 }
 
 // Merges the key chunks of a query row: out = v_scale * sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c.
-// A warp per row; `block_rows` rows per unit in the workspace.
-__global__ void __launch_bounds__(128) kv4_combine_kernel(const __grid_constant__ AParams p, int block_rows) {
+// A warp per row.
+__global__ void __launch_bounds__(128) kv4_combine_kernel(const __grid_constant__ AParams p) {
+  constexpr int R = kBlockRows;
   const int lane = threadIdx.x & 31;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   const int64_t bh = at / p.rows;  // (member, K/V head)
   if (bh >= p.units / p.row_blocks) return;
   const int row = static_cast<int>(at - bh * p.rows);
-  const int rb = row / block_rows;
-  const int64_t slot0 = (bh * p.row_blocks + rb) * p.chunks * block_rows + (row - rb * block_rows);
+  const int b = static_cast<int>(bh / p.cache.kv_heads), h = static_cast<int>(bh % p.cache.kv_heads);
+  const int rb = row / R;
   pdl_wait();
+  int before = b * p.chunks, chunks = p.chunks;
+  if (chunks == 0) {
+    const int4 info = p.ws_units[b];
+    before = info.x;
+    chunks = info.y;
+    if (chunks == 1) return;  // the rows kernel wrote the row
+  }
+  const int64_t first = static_cast<int64_t>(before) * p.cache.kv_heads + static_cast<int64_t>(h) * chunks;
+  const int64_t slot0 = (first * p.row_blocks + rb) * R + (row - rb * R), step = static_cast<int64_t>(p.row_blocks) * R;
   float top = -INFINITY;
   float2 ml[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int ch = lane + 32 * i;
-    ml[i] = ch < p.chunks ? p.ws_ml[slot0 + static_cast<int64_t>(ch) * block_rows] : make_float2(-INFINITY, 0.f);
+    ml[i] = ch < chunks ? p.ws_ml[slot0 + ch * step] : make_float2(-INFINITY, 0.f);
     top = fmaxf(top, ml[i].x);
   }
 #pragma unroll
@@ -524,18 +619,23 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const __grid_constant_
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   const float* src = p.ws_o + slot0 * kKv4D + 4 * lane;
-#pragma unroll 4
-  for (int ch = 0; ch < p.chunks; ++ch) {
-    const float w = __shfl_sync(0xffffffffu, ch < 32 ? f[0] : f[1], ch & 31);
-    if (w == 0.f) continue;  // a chunk in which the row saw nothing (its sums may not have been written)
-    const float4 y = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(ch) * block_rows * kKv4D);
-    x.x += w * y.x;
-    x.y += w * y.y;
-    x.z += w * y.z;
-    x.w += w * y.w;
+  // 16 chunks at a time, so that their loads are in flight together.
+  for (int c0 = 0; c0 < chunks; c0 += 16) {
+    float4 y[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      y[i] = *reinterpret_cast<const float4*>(src + min(c0 + i, chunks - 1) * step * kKv4D);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float w = __shfl_sync(0xffffffffu, c0 < 32 ? f[0] : f[1], (c0 + i) & 31);
+      if (w == 0.f) continue;  // behind the last chunk, or a chunk in which the row saw nothing
+      x.x += w * y[i].x;
+      x.y += w * y[i].y;
+      x.z += w * y[i].z;
+      x.w += w * y[i].w;
+    }
   }
   const float inv = sum == 0.f ? 0.f : p.cache.v_scale / sum;
-  const int b = static_cast<int>(bh / p.cache.kv_heads), h = static_cast<int>(bh % p.cache.kv_heads);
   const int t = row / p.group;
   __nv_bfloat16* dst = p.out + b * p.out_member + t * p.out_row + (h * p.group + (row - t * p.group)) * kKv4D + 4 * lane;
   *reinterpret_cast<uint2*>(dst) = make_uint2(Pairs16<__nv_bfloat16>::pack_pair(x.x * inv, x.y * inv),
@@ -1287,7 +1387,7 @@ __global__ void __launch_bounds__(256) kv4_merge_kernel(const __grid_constant__ 
 struct APlan {
   AParams params;
   int kernel;       // ps_kv4_kernel, resolved
-  int block_rows;   // query rows of a block (workspace)
+  int64_t ctas;     // rows kernel: grid
   int64_t ws_bytes;
 };
 
@@ -1343,6 +1443,7 @@ static int build_attn(const ps_kv4_attn_args* a, APlan* plan, bool host_only) {
   if (a->kv_tokens > a->cache.table_pages * a->cache.page_rows)
     return fail(PS_ERR_BOUNDS, "kv_tokens=%d exceeds a member's %lld cache rows", a->kv_tokens,
                 (long long)(a->cache.table_pages * a->cache.page_rows));
+  if (a->kv_tokens > (1 << 30)) return fail(PS_ERR_UNSUPPORTED, "kv_tokens=%d beyond 2^30", a->kv_tokens);
   if (a->kernel != PS_KV4_AUTO && a->kernel != PS_KV4_ROWS && a->kernel != PS_KV4_TILES)
     return fail(PS_ERR_SHAPE, "kernel %d unknown", a->kernel);
   if (a->key_chunks < 0 || a->key_chunks > kMaxChunks)
@@ -1379,8 +1480,8 @@ static int build_attn(const ps_kv4_attn_args* a, APlan* plan, bool host_only) {
     plan->kernel = rows_us <= tiles_us ? PS_KV4_ROWS : PS_KV4_TILES;
   }
   const bool tiles_kernel = plan->kernel == PS_KV4_TILES;
-  plan->block_rows = tiles_kernel ? kUnitRows : kBlockRows;
-  p.row_blocks = (p.rows + plan->block_rows - 1) / plan->block_rows;
+  const int block_rows = tiles_kernel ? kUnitRows : kBlockRows;
+  p.row_blocks = (p.rows + block_rows - 1) / block_rows;
   if (p.row_blocks > 0 && a->cache.members * hk > (1 << 26) / p.row_blocks)
     return fail(PS_ERR_UNSUPPORTED, "%lld members of %d K/V heads and %d row blocks", (long long)a->cache.members, hk,
                 p.row_blocks);
@@ -1401,10 +1502,22 @@ static int build_attn(const ps_kv4_attn_args* a, APlan* plan, bool host_only) {
     int chunks = a->key_chunks > 0 ? a->key_chunks : choose_chunks(p.units, tiles, 3ll * sms);
     if (chunks > tiles) chunks = tiles > 0 ? tiles : 1;
     p.chunks = chunks;
-    slots = p.units * p.chunks * plan->block_rows;
-    plan->ws_bytes = p.chunks > 1 ? slots * (kKv4D * 4 + 8) : 0;
+    plan->ctas = p.units * chunks;
+    if (a->kv_lens && a->key_chunks == 0 && chunks > 1 && p.units <= sms) {
+      // Few units of work of lengths that the host does not know: the device splits them by length.  One wave
+      // of CTAs, or up to four while a chunk keeps a dozen tiles (of windows half as long as they may be).
+      // 7 members x 12 rows of 8 K/V heads over 1 024 .. 8 191 keys (112 units): 26 us, equal chunks 30.  With
+      // more units than SMs the waves even the lengths out by themselves, and the split only costs its
+      // planning (200 units of 375 .. 3 000 keys: 27.3 us, equal chunks 26.4).
+      const int64_t wave = 3ll * sms, waves = p.units * tiles / (2 * wave * 12);
+      p.chunks = 0;
+      plan->ctas = wave * (waves < 1 ? 1 : waves > 4 ? 4 : waves);
+    }
+    slots = plan->ctas * kBlockRows;
+    plan->ws_bytes = chunks > 1 ? slots * (kKv4D * 4 + 8) : 0;
+    if (p.chunks == 0) plan->ws_bytes += a->cache.members * static_cast<int64_t>(sizeof(int4));
   }
-  if (p.units * p.chunks > 0x7fffffffLL) return fail(PS_ERR_UNSUPPORTED, "grid of %lld CTAs", (long long)(p.units * p.chunks));
+  if (plan->ctas > 0x7fffffffLL) return fail(PS_ERR_UNSUPPORTED, "grid of %lld CTAs", (long long)plan->ctas);
   if (!host_only && plan->ws_bytes > 0) {
     if (!a->workspace || a->workspace_bytes < plan->ws_bytes)
       return fail(PS_ERR_NULL, "workspace of %lld bytes needed (ps_kv4_attention_workspace), %lld given",
@@ -1489,10 +1602,10 @@ extern "C" int32_t ps_attention_kv4(const ps_kv4_attn_args* args, void* stream) 
   }
   const int smem = static_cast<int>(sizeof(ps::RowsShared)) + 128;
   cudaError_t err = ps::allow_smem(reinterpret_cast<const void*>(ps::kv4_rows_kernel), smem);
-  if (err == cudaSuccess) err = ps::launch(ps::kv4_rows_kernel, p.units * p.chunks, ps::kRowThreads, smem, s, p);
-  if (err == cudaSuccess && p.chunks > 1) {
+  if (err == cudaSuccess) err = ps::launch(ps::kv4_rows_kernel, plan.ctas, ps::kRowThreads, smem, s, p);
+  if (err == cudaSuccess && p.chunks != 1) {
     const int64_t rows = p.units / p.row_blocks * p.rows;
-    err = ps::launch(ps::kv4_combine_kernel, (rows + 3) / 4, 128, 0, s, p, plan.block_rows);
+    err = ps::launch(ps::kv4_combine_kernel, (rows + 3) / 4, 128, 0, s, p);
   }
   if (err != cudaSuccess) return ps::fail(PS_ERR_LAUNCH, "kv4 attention launch: %s", cudaGetErrorString(err));
   return PS_OK;

@@ -1008,7 +1008,8 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, kv_
     lib = _lib.load()
     with _on_device(device_index):
         # The size of the partial results depends on the shape of the call alone: asked once per shape.
-        shape = (device_index, heads, Lq, most, causal_block, code, key_chunks, members, table.shape[1], pages.shape[1])
+        shape = (device_index, heads, Lq, most, causal_block, code, key_chunks, members, table.shape[1], pages.shape[1],
+                 lens != 0)
         need = _ATTN4_NEED.get(shape)
         if need is None:
             asked = ctypes.c_int64(0)

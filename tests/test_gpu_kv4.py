@@ -398,6 +398,24 @@ def test_attention_ragged_lengths(Lq, cb, chunks, kernel):
     check_attention(short, q, k, v, [min(max(n, 0), 300) for n in lens], 4, cb)
 
 
+@pytest.mark.parametrize("members,Lq,heads,hk,cb,rows", [
+    (5, 3, 4, 2, 1, 6000),      # two row blocks, long and short windows
+    (40, 1, 2, 2, 0, 1500),     # more members than a warp has lanes
+    (1, 1, 3, 3, 0, 8191),
+    (2, 20, 2, 1, 7, 3000),
+])
+@pytest.mark.parametrize("lens", ["spread", "equal", "one", "none"])
+def test_attention_splits_the_keys_by_the_lengths(members, Lq, heads, hk, cb, rows, lens):
+    """Few units of work whose lengths only the device knows: chunks of like length, whatever the lengths are."""
+    pages, table, k, v = fill(members, rows, hk, 64, 31)
+    q = torch.randn(members, Lq, heads * 128, generator=gen(32)).bfloat16()
+    ns = {"spread": torch.randint(0, rows + 1, (members,), generator=gen(33)), "equal": torch.full((members,), rows),
+          "one": torch.where(torch.arange(members) == members - 1, rows, 1), "none": torch.zeros(members)}[lens].int()
+    dev = ops.attention_kv4(q.to(DEV), pages.to(DEV), table.to(DEV), ns.to(DEV), heads=heads, causal_block=cb, kernel="rows",
+                            max_kv_tokens=rows)
+    check_attention(dev, q, k, v, ns.tolist(), heads, cb)
+
+
 @pytest.mark.parametrize("kernel", ["rows", "tiles"])
 @pytest.mark.parametrize("Lq", [1, 200])
 def test_attention_never_reads_behind_the_window(Lq, kernel):
