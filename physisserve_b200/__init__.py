@@ -10,7 +10,10 @@ into the same-step noisy-KV history -- as hand-written CUDA kernels behind a C A
   (wan.py:85-111), pre-RoPE pages and window tables unchanged;
 * ``physisserve_b200.wan.prep_ring`` / ``RingCache`` / ``RingAttention`` -- the ring
   layout: rotated K/V written once at ring slot, sink re-rotated when it moves;
-* ``physisserve_b200.ops.qk_norm_rope_kv`` -- the fused kernel itself.
+* ``physisserve_b200.ops.qk_norm_rope_kv`` -- the fused kernel itself;
+* ``physisserve_b200.ops.qk_norm_rope_kv4`` / ``read_kv4`` / ``attention_kv4`` and
+  ``physisserve_b200.wan.RingCache4`` -- the same with the K/V history in 4 bits an element, in
+  pages of a shared pool (``include/physis_b200_kv4.h``).
 """
 from . import _lib
 

@@ -7,7 +7,8 @@
 //   at the same 16 columns of its heads, so it reads one slice of the rotation tables.
 //
 //   Bound: HBM, 9.125 C bytes a token (C = heads * 128, kv_heads = heads, bf16), against 12 C of the
-//   bf16 ring; but the quantisation adds arithmetic, so issue slots come second by little.
+//   bf16 ring.  Measured: 12 480 tokens of 40 heads in 150 us, 60 % of the copy bandwidth: about 7 400
+//   warp instructions a token at 0.6 a clock and scheduler are what the time goes to.
 //
 //   K's sum of squares is accumulated in fp64: bf16 squares are exact there and so is their sum, so
 //   the row's 1/sqrt -- and every rounding of what is quantised -- does not depend on the order of
@@ -16,7 +17,8 @@
 //   the conversion unit.  Q's sum stays fp32: nothing that it moves is quantised.
 //
 // kv4_read_kernel -- rows back as bf16 or fp32: a thread expands 8 code bytes and a scale of K and
-//   of V to 16 numbers each (one 256-bit store each in bf16).  Bound: HBM, mostly by the writes.
+//   of V to 16 numbers each (one 256-bit store each in bf16).  Bound: HBM, mostly by the writes; 34 320
+//   rows of 12 heads in 45.5 us, 92 % of the copy bandwidth.
 
 #include <stdio.h>
 #include <string.h>

@@ -612,13 +612,14 @@ def qk_norm_rope_tables(
 def _member_rows(t: torch.Tensor, C: int, name: str):
     """(member stride, row stride) in elements of a [B, rows, C] or [B, rows, H, D] tensor whose
     rows are contiguous C-element vectors."""
-    if t.dim() == 4:
-        if t.shape[2] * t.shape[3] != C or t.stride(3) != 1 or t.stride(2) != t.shape[3]:
-            raise PrepError(f"{name}: [B, rows, H, D] with contiguous heads expected, got {tuple(t.shape)}")
-    elif t.dim() != 3 or t.shape[2] != C or t.stride(2) != 1:
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 4:
+        if shape[2] * shape[3] != C or stride[3] != 1 or stride[2] != shape[3]:
+            raise PrepError(f"{name}: [B, rows, H, D] with contiguous heads expected, got {tuple(shape)}")
+    elif len(shape) != 3 or shape[2] != C or stride[2] != 1:
         raise PrepError(f"{name}: [B, rows, {C}] with unit stride on the last dimension expected, got "
-                        f"{tuple(t.shape)}")
-    return t.stride(0), t.stride(1)
+                        f"{tuple(shape)}")
+    return stride[0], stride[1]
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_tokens: int | None = None, *,
@@ -710,12 +711,13 @@ def kv4_pages(num_pages: int, kv_heads: int, page_rows: int = 128, device=None) 
 
 def _kv4_cache(pages: torch.Tensor, table: torch.Tensor, k_scale: float, v_scale: float):
     """(device index, members, page_rows, ``ps_kv4_cache`` fields) of a pool and a page table."""
-    if pages.dtype is not torch.uint8 or pages.dim() != 4 or pages.shape[2] != 2 or not pages.is_contiguous():
+    shape = pages.shape
+    if pages.dtype is not torch.uint8 or len(shape) != 4 or shape[2] != 2 or not pages.is_contiguous():
         raise PrepError("pages must be a contiguous uint8 [pages, kv_heads, 2, page_rows * 72] tensor, got "
-                        f"{pages.dtype} {tuple(pages.shape)}")
-    page_rows, rest = divmod(pages.shape[3], KV4_ROW_BYTES)
+                        f"{pages.dtype} {tuple(shape)}")
+    page_rows, rest = divmod(shape[3], KV4_ROW_BYTES)
     if rest or page_rows not in KV4_PAGE_ROWS:
-        raise PrepError(f"pages of {pages.shape[3]} bytes a head: page_rows * {KV4_ROW_BYTES} with page_rows one of "
+        raise PrepError(f"pages of {shape[3]} bytes a head: page_rows * {KV4_ROW_BYTES} with page_rows one of "
                         f"{KV4_PAGE_ROWS}")
     if table.dtype is not torch.int32 or table.dim() != 2 or not table.is_contiguous():
         raise PrepError(f"table must be a contiguous int32 [members, pages] tensor, got {table.dtype} "
@@ -728,8 +730,8 @@ def _kv4_cache(pages: torch.Tensor, table: torch.Tensor, k_scale: float, v_scale
     if not (1e-20 <= k_scale <= 1e20 and 1e-20 <= v_scale <= 1e20):
         raise PrepError(f"tensor scales {k_scale} and {v_scale} outside [1e-20, 1e20]")
     members, table_pages = table.shape
-    return device_index, members, page_rows, (pages.data_ptr(), table.data_ptr(), pages.shape[0], members, table_pages,
-                                              pages.shape[1], page_rows, k_scale, v_scale)
+    return device_index, members, page_rows, (pages.data_ptr(), table.data_ptr(), shape[0], members, table_pages,
+                                              shape[1], page_rows, k_scale, v_scale)
 
 
 def _prepare4(
@@ -915,9 +917,10 @@ def read_kv4(pages: torch.Tensor, table: torch.Tensor, tokens: int, *, row0: int
     ordinary window.  ``k_out``/``v_out`` receive them if given (their dtype is then used).  Rows of pages
     outside the pool read as zero and are counted in ``kv4_counters``."""
     device_index, members, _, cache = _kv4_cache(pages, table, k_scale, v_scale)
-    C = pages.shape[1] * KV4_HEAD_DIM
+    C = cache[5] * KV4_HEAD_DIM
     tokens, row0 = int(tokens), int(row0)
-    dtype = next((t.dtype for t in (k_out, v_out) if t is not None), dtype)
+    if k_out is not None or v_out is not None:
+        dtype = v_out.dtype if k_out is None else k_out.dtype
     code = _DEVICE_DTYPES.get(dtype)
     if code is None:
         raise PrepError(f"unsupported dtype {dtype}: the kernels write bfloat16 or float32")
@@ -926,7 +929,9 @@ def read_kv4(pages: torch.Tensor, table: torch.Tensor, tokens: int, *, row0: int
     outs, strides = [], []
     for name, t in (("k_out", k_out), ("v_out", v_out)):
         if t is None:
-            outs.append(torch.empty(members, tokens, C, dtype=dtype, device=pages.device))
+            # (like the first one: half a microsecond less than naming the type and the device again)
+            outs.append(torch.empty_like(outs[0], memory_format=torch.contiguous_format) if outs else
+                        torch.empty(members, tokens, C, dtype=dtype, device=pages.device))
             strides.append((tokens * C, C))
             continue
         if t.dtype is not dtype or t.get_device() != device_index:
@@ -970,14 +975,14 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, kv_
         raise PrepError("attention takes bfloat16 q")
     if q.get_device() != device_index:
         raise PrepError(f"q is on {q.device}, the cache on {pages.device}")
-    C = heads * KV4_HEAD_DIM
-    if q.dim() < 3 or q.shape[0] != members:
-        raise PrepError(f"q must be [{members}, Lq, {C}], got {tuple(q.shape)}")
-    Lq = q.shape[1]
+    C, q_shape = heads * KV4_HEAD_DIM, q.shape
+    if len(q_shape) < 3 or q_shape[0] != members:
+        raise PrepError(f"q must be [{members}, Lq, {C}], got {tuple(q_shape)}")
+    Lq = q_shape[1]
     code = _KV4_KERNELS.get(kernel)
     if code is None:
         raise PrepError(f"kernel {kernel!r} is not one of {sorted(_KV4_KERNELS)}")
-    rows, lens = table.shape[1] * page_rows, 0
+    rows, lens = cache[4] * page_rows, 0
     # (kv_tokens keeps its name: a lengths tensor that the caller made for this call alone must live until
     # the launch, or `out` could be allocated in its memory.)
     if kv_tokens is None:
@@ -996,7 +1001,7 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, kv_
     qs = _member_rows(q, C, "q")
     if out is None:
         out, os_ = torch.empty(members, Lq, C, device=q.device, dtype=torch.bfloat16), (Lq * C, C)
-    elif out.dtype is not torch.bfloat16 or out.get_device() != device_index or out.shape[:2] != q.shape[:2]:
+    elif out.dtype is not torch.bfloat16 or out.get_device() != device_index or out.shape[:2] != q_shape[:2]:
         raise PrepError(f"out must be a bfloat16 [{members}, {Lq}, {C}] tensor on {pages.device}")
     else:
         os_ = _member_rows(out, C, "out")
@@ -1008,7 +1013,7 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, kv_
     lib = _lib.load()
     with _on_device(device_index):
         # The size of the partial results depends on the shape of the call alone: asked once per shape.
-        shape = (device_index, heads, Lq, most, causal_block, code, key_chunks, members, table.shape[1], pages.shape[1],
+        shape = (device_index, heads, Lq, most, causal_block, code, key_chunks, members, cache[4], cache[5],
                  lens != 0)
         need = _ATTN4_NEED.get(shape)
         if need is None:
