@@ -158,7 +158,8 @@ PS_API int32_t ps_kv4_read_validate(const ps_kv4_read_args* args);
  * are rounded to fp16 for P V; the output is rounded once to bf16. */
 PS_API int32_t ps_attention_kv4(const ps_kv4_attn_args* args, void* stream);
 PS_API int32_t ps_kv4_attention_validate(const ps_kv4_attn_args* args);
-/* Bytes of scratch that ps_attention_kv4 needs for these arguments on the current device. */
+/* Bytes of scratch that ps_attention_kv4 needs for these arguments on the current device (of the pointers
+ * only kv_lens matters: whether it is NULL). */
 PS_API int32_t ps_kv4_attention_workspace(const ps_kv4_attn_args* args, int64_t* bytes);
 
 /* Counts on the current device since the last reset: counts[0] accesses to pages
