@@ -681,12 +681,19 @@ static int build_prep(const ps_kv4_prep_args* a, PPlan* plan) {
   plan->dtype = a->dtype;
   int warps = 1;
   plan->nb = 1;
-  // A launch whose tokens are all resident at once with one block a thread (20 warps an SM) is bound by the time
-  // of a token, not by throughput: then one block a thread (8 tokens of 12 heads 3.2 us against 5.7, 800 tokens
-  // 6.0 against 7.5, 200 tokens of 40 heads 6.5 against 10.4; past it 1 560 tokens of 12 heads 10.4 against 8.6).
+  // A launch whose tokens are all resident at once (18 warps an SM) is bound by the time of a token, not by
+  // throughput: then one block a thread, or two of bf16, whichever come to fit first.  8 tokens of 12 heads 3.2 us
+  // against 5.7, 800 tokens 6.0 against 7.5, 400 tokens of 40 heads 7.7 against 10.7; past it 1 560 tokens of 12
+  // heads 10.4 (one block) against 8.6.
   const int most = a->heads > hk ? a->heads : hk;
-  const bool few = total * ((most + 3) / 4) <= 148 * 20;
-  choose_split(most, few && (most + 3) / 4 * 32 <= kMaxTpt ? 1 : max_blocks(a->dtype), &plan->nb, &warps);
+  choose_split(most, max_blocks(a->dtype), &plan->nb, &warps);
+  for (int n = a->dtype == PS_BF16 ? 2 : 1; n >= 1; --n) {
+    const int w = (most + 4 * n - 1) / (4 * n);
+    if (n < plan->nb && w * 32 <= kMaxTpt && total * w <= 148 * 18) {
+      plan->nb = n;
+      warps = w;
+    }
+  }
   p.tpt = warps * 32;
   p.hstep = warps * 4;
   p.tokens_cta = warps == 1 ? 2 : 1;

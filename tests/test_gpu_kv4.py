@@ -137,6 +137,21 @@ def test_append_matches_the_definition_bit_for_bit(case, fused):
     assert ops.kv4_counters() == (0, 0, 0)
 
 
+@pytest.mark.parametrize("case", [
+    (1, 34, 42, 1, 12, 12, 128, torch.bfloat16, 1),     # more tokens than are resident: three blocks a thread
+    (1, 34, 80, 1, 16, 4, 64, torch.bfloat16, 1),       # four
+    (2, 34, 42, 1, 20, 3, 32, torch.bfloat16, 1),       # five, one warp a token
+    (1, 23, 41, 1, 33, 33, 16, torch.bfloat16, 1),      # several warps, the last one with heads missing
+    (1, 34, 42, 1, 12, 12, 128, torch.float32, 1),
+    (1, 52, 52, 1, 7, 2, 16, torch.float32, 1),
+])
+def test_append_of_many_tokens(case):
+    kwargs, want, q_ref, _ = append_case(*case, seed=case[4])
+    ops.qk_norm_rope_kv4(**kwargs)
+    assert torch.equal(kwargs["pages"].cpu(), want)
+    check_q(kwargs["q_out"], q_ref, case[7])
+
+
 @pytest.mark.parametrize("k_scale,v_scale,size", [(0.37, 1.7, 1.0), (1e-3, 2.0 ** -20, 30.0), (1e4, 1e6, 1.0),
                                                   (1e-20, 1e20, 1.0)])
 def test_append_tensor_scales(k_scale, v_scale, size):
