@@ -634,6 +634,25 @@ def test_a_captured_decoding_step_appends_and_attends():
         check_attention(outs[t], q.view(members, 1, -1), k[:, :t + 1], v[:, :t + 1], [t + 1] * members, heads)
 
 
+def test_one_workspace_for_calls_of_unlike_shapes():
+    """The caller's scratch, full of ones, for calls of both kernels one after another: nothing of it is taken for
+    the call's own."""
+    workspace = torch.full((1 << 27,), 0xff, dtype=torch.uint8, device=DEV)
+    calls = []
+    for members, Lq, heads, hk, rows, kernel in ((3, 2, 4, 2, 2500, "rows"), (2, 300, 2, 2, 900, "tiles"), (1, 1, 2, 1, 4000, "rows"),
+                                                 (5, 130, 4, 4, 260, "tiles"), (6, 1, 2, 2, 1200, "rows")):
+        pages, table, k, v = fill(members, rows, hk, 32, rows)
+        q = torch.randn(members, Lq, heads * 128, generator=gen(Lq)).bfloat16()
+        lens = torch.randint(0, rows + 1, (members,), generator=gen(rows)).int()
+        calls.append((q, k, v, lens, heads, dict(q=q.to(DEV), pages=pages.to(DEV), table=table.to(DEV), heads=heads,
+                                                 max_kv_tokens=rows, kernel=kernel, workspace=workspace)))
+    lens_dev = [c[3].to(DEV) for c in calls]
+    for _ in range(2):
+        outs = [ops.attention_kv4(kv_tokens=n, **c[5]) for n, c in zip(lens_dev, calls)]
+    for out, (q, k, v, lens, heads, _) in zip(outs, calls):
+        check_attention(out, q, k, v, lens.tolist(), heads)
+
+
 def test_results_do_not_depend_on_the_run():
     pages, table, _, _ = fill(2, 2000, 2, 64, 16)
     for Lq in (1, 300):
