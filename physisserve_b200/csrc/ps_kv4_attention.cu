@@ -1487,7 +1487,7 @@ static int build_attn(const ps_kv4_attn_args* a, APlan* plan, bool host_only) {
   const bool tiles_kernel = plan->kernel == PS_KV4_TILES;
   const int block_rows = tiles_kernel ? kUnitRows : kBlockRows;
   p.row_blocks = (p.rows + block_rows - 1) / block_rows;
-  if (p.row_blocks > 0 && a->cache.members * hk > (1 << 26) / p.row_blocks)
+  if (p.row_blocks > 0 && a->cache.members * hk > (1 << 25) / p.row_blocks)
     return fail(PS_ERR_UNSUPPORTED, "%lld members of %d K/V heads and %d row blocks", (long long)a->cache.members, hk,
                 p.row_blocks);
   p.units = a->cache.members * hk * p.row_blocks;

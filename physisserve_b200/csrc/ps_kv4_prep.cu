@@ -428,7 +428,6 @@ struct RParams {
   int64_t k_member, k_row, v_member, v_row;  // element strides
   int64_t row0;
   uint64_t rows_magic;   // div_magic(rows)
-  int64_t member_rows;   // logical rows per member
   uint32_t rows;
   uint32_t items;        // members * rows * kv_heads * 8
   uint64_t per_magic;    // div_magic(kv_heads * 8)
@@ -770,7 +769,6 @@ static int build_read(const ps_kv4_read_args* a, RParams* p) {
   p->row0 = a->row0;
   p->rows = static_cast<uint32_t>(a->rows);
   p->rows_magic = div_magic(p->rows);
-  p->member_rows = member_rows;
   p->per = static_cast<uint32_t>(per);
   p->per_magic = div_magic(p->per);
   p->items = static_cast<uint32_t>(a->cache.members * a->rows * per);
