@@ -326,11 +326,13 @@ class RingCache4:
         self.table.fill_(-1)
         self.sink_at = [None] * self.batch
 
-    def window(self, chunk: int):
-        """(K, V) windows [batch, heads, tokens, head_dim] of ``chunk``, read back in the activation dtype."""
+    def window(self, chunk: int, member: int | None = None):
+        """(K, V) windows [batch, heads, tokens, head_dim] of ``chunk``, read back in the activation dtype;
+        of one member (batch 1) if given, for members whose windows are unlike."""
         n = self.window_rows(chunk)
-        k, v = read_kv4(self.pages, self.table, n, k_scale=self.k_scale, v_scale=self.v_scale, dtype=self.sink_k.dtype)
-        shape = (self.batch, n, self.heads, self.head_dim)
+        table = self.table if member is None else self.table[member:member + 1]
+        k, v = read_kv4(self.pages, table, n, k_scale=self.k_scale, v_scale=self.v_scale, dtype=self.sink_k.dtype)
+        shape = (table.shape[0], n, self.heads, self.head_dim)
         return k.view(shape).transpose(1, 2), v.view(shape).transpose(1, 2)
 
 
@@ -455,8 +457,11 @@ class RingAttention:
         else:
             outs = []
             for b, pos in enumerate(positions):
-                kw, vw = cache.window(pos.chunk)
-                outs.append(F.scaled_dot_product_attention(q_rot[b:b + 1], kw[b:b + 1], vw[b:b + 1]))
+                if isinstance(cache, RingCache4):
+                    kw, vw = cache.window(pos.chunk, b)
+                else:
+                    kw, vw = (x[b:b + 1] for x in cache.window(pos.chunk))
+                outs.append(F.scaled_dot_product_attention(q_rot[b:b + 1], kw, vw))
             out = torch.cat(outs)
         hidden = out.transpose(1, 2).flatten(2)
         return attn.to_out[1](attn.to_out[0](hidden))

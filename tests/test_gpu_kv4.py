@@ -807,3 +807,28 @@ def test_ring_processor_members_at_different_chunks():
             check_attention(got, q_rot, k.cpu().double().view(2, n, heads, 128), v.cpu().double().view(2, n, heads, 128), lens,
                             heads)
     ops.kv4_counters()
+
+
+def test_unlike_windows_read_back_touch_their_own_pages():
+    """SDPA over windows of unlike length: a member's read asks for the pages that it holds, no others."""
+    from physisserve_b200.wan import RingAttention, RingCache4, wan_rope_tables, window_layout
+
+    torch.manual_seed(2)
+    heads, gh, gw = 2, 2, 4
+    C, hw = heads * 128, gh * gw
+    attn = FakeAttn(heads, C).to(DEV, torch.bfloat16)
+    cos, sin = wan_rope_tables(128, 64, device=DEV)
+    cache = RingCache4(heads=heads, grid_h=gh, grid_w=gw, batch=2, page_rows=16, device=DEV)
+    proc, sdpa = RingAttention(), RingAttention(attention_kernel=False)
+    proc.cache = sdpa.cache = cache
+    ops.kv4_counters()
+    with torch.no_grad():
+        proc(attn, torch.randn(2, 3 * hw, C, device=DEV).bfloat16(), rotary_emb=(cos, sin, [window_layout(0)] * 2))
+        for chunks in ((1, 1), (2, 1), (3, 1), (4, 1)):
+            rotary = (cos, sin, [window_layout(c) for c in chunks])
+            x = torch.randn(2, hw, C, device=DEV).bfloat16()
+            got, again = proc(attn, x, rotary_emb=rotary), sdpa(attn, x, rotary_emb=rotary)
+            assert float((again.float() - got.float()).abs().max()) <= 2 ** -5 * float(got.float().abs().max())
+    assert ops.kv4_counters().bad_pages == 0
+    k, _ = cache.window(4, 0)
+    assert k.shape == (1, heads, cache.window_rows(4), 128)
