@@ -133,7 +133,7 @@ typedef struct ps_kv4_attn_args {
   const void* q;  int64_t q_member_stride;   int64_t q_row_stride;   /* bf16 */
   void* out;      int64_t out_member_stride; int64_t out_row_stride; /* bf16 */
   const int32_t* kv_lens; /* device [members], or NULL */
-  void* workspace;        /* device scratch of ps_kv4_attention_workspace() bytes */
+  void* workspace;        /* device scratch of ps_kv4_attention_workspace() bytes, 16-byte aligned */
   int64_t workspace_bytes;
   ps_kv4_cache cache;
 } ps_kv4_attn_args;

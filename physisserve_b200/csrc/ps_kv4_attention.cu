@@ -34,7 +34,8 @@ struct AParams {
   int32_t min_steps;     // tiles kernel: fewest steps of a CTA
   int64_t units;         // members * kv_heads * row_blocks
   float scale_log2;      // softmax scale * k_scale * log2(e)
-  float* ws_o;           // partial results: [slots][rows of a block][128] unnormalised sums,
+  float* ws_o;           // partial results: [slots][rows of a block][128] unnormalised sums (32-byte aligned in the
+                         // tiles kernel, which stores 32 bytes at a time),
   float2* ws_ml;         // [slots][rows of a block] (reference in log2 units, sum); slots are
                          // [CTAs] (rows kernel) or [grid][2] (tiles kernel)
   int4* ws_units;        // tiles kernel: [units] (first CTA, last CTA, the first CTA's slot, 0);
@@ -1502,7 +1503,8 @@ static int build_attn(const ps_kv4_attn_args* a, APlan* plan, bool host_only) {
     const int64_t most = p.units * (tiles > 0 ? tiles : 1);
     if ((most + p.min_steps - 1) / p.min_steps < p.grid) p.grid = static_cast<int32_t>((most + p.min_steps - 1) / p.min_steps);
     slots = 2ll * p.grid * kUnitRows;
-    plan->ws_bytes = slots * (kKv4D * 4 + 8) + p.units * static_cast<int64_t>(sizeof(int4));
+    // The partial rows go out 32 bytes at a time: they start at the workspace's first 32-byte boundary.
+    plan->ws_bytes = slots * (kKv4D * 4 + 8) + p.units * static_cast<int64_t>(sizeof(int4)) + 16;
   } else {
     int chunks = a->key_chunks > 0 ? a->key_chunks : choose_chunks(p.units, tiles, 3ll * sms);
     if (chunks > tiles) chunks = tiles > 0 ? tiles : 1;
@@ -1529,8 +1531,10 @@ static int build_attn(const ps_kv4_attn_args* a, APlan* plan, bool host_only) {
                   (long long)plan->ws_bytes, (long long)a->workspace_bytes);
     if (!aligned16(a->workspace)) return fail(PS_ERR_ALIGN, "workspace is not 16-byte aligned");
   }
-  p.ws_o = static_cast<float*>(a->workspace);
-  p.ws_ml = reinterpret_cast<float2*>(static_cast<unsigned char*>(a->workspace) + slots * kKv4D * 4);
+  unsigned char* base = static_cast<unsigned char*>(a->workspace);
+  if (tiles_kernel && (reinterpret_cast<uintptr_t>(base) & 31u)) base += 16;
+  p.ws_o = reinterpret_cast<float*>(base);
+  p.ws_ml = reinterpret_cast<float2*>(base + slots * kKv4D * 4);
   p.ws_units = reinterpret_cast<int4*>(p.ws_ml + slots);
   return PS_OK;
 }

@@ -14,11 +14,13 @@ bf16, 2^-8 |out|; each p's rounding to fp16, 2^-11 relative and so 2^-11 A; each
 approximate 2^x (2^-22), together below 2^-13 A; a p below fp16's normal range loses at most 2^-25 absolutely
 against a largest p of at least 1, N keys together 2^-25 N max|v|.  Tolerance: 2^-8 |out| + 2^-10 A + 2^-24 N max|v|.
 """
+import ctypes
+
 import pytest
 import torch
 
 from oracle import kv4, wan_prep
-from physisserve_b200 import ops
+from physisserve_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -832,3 +834,36 @@ def test_unlike_windows_read_back_touch_their_own_pages():
     assert ops.kv4_counters().bad_pages == 0
     k, _ = cache.window(4, 0)
     assert k.shape == (1, heads, cache.window_rows(4), 128)
+
+
+# ---------------------------------------------------------------------------------------
+# The caller's workspace
+# ---------------------------------------------------------------------------------------
+def workspace_bytes(q, pages, table, rows, heads, kernel, lens=0):
+    """What ps_kv4_attention_workspace reports for a call of contiguous tensors."""
+    args = _lib.PsKv4AttnArgs(heads=heads, q_tokens=q.shape[1], kv_tokens=rows, kernel=kernel, q=q.data_ptr(),
+                              q_member_stride=q.stride(0), q_row_stride=q.stride(1), out=q.data_ptr(),
+                              out_member_stride=q.stride(0), out_row_stride=q.stride(1), kv_lens=lens,
+                              cache=_lib.PsKv4Cache(*ops._kv4_cache(pages, table, 1.0, 1.0)[3]))
+    need = ctypes.c_int64(0)
+    assert _lib.load().ps_kv4_attention_workspace(ctypes.byref(args), ctypes.byref(need)) == _lib.OK
+    return need.value
+
+
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
+@pytest.mark.parametrize("offset", [0, 16, 32, 48])
+def test_attention_workspace_on_any_16_byte_boundary(kernel, offset):
+    """The scratch cut out of a larger buffer: no byte outside of it is written."""
+    rows, Lq = 2500, 3 if kernel == "rows" else 300
+    pages, table, k, v = fill(1, rows, 2, 128, 61)
+    q = torch.randn(1, Lq, 256, generator=gen(62)).bfloat16()
+    dev = q.to(DEV), pages.to(DEV), table.to(DEV)
+    need = workspace_bytes(*dev, rows, 2, {"rows": _lib.KV4_ROWS, "tiles": _lib.KV4_TILES}[kernel])
+    assert need > 0
+    arena = torch.full((offset + need + 64,), 0x5a, dtype=torch.uint8, device=DEV)
+    workspace = arena[offset:offset + need]
+    assert workspace.data_ptr() % 64 == offset
+    got = ops.attention_kv4(*dev, rows, heads=2, kernel=kernel, workspace=workspace)
+    check_attention(got, q, k, v, [rows], 2)
+    assert bool((arena[:offset] == 0x5a).all()) and bool((arena[offset + need:] == 0x5a).all())
+    assert not bool((workspace == 0x5a).all())

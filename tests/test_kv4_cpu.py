@@ -287,3 +287,21 @@ def test_ring_cache_refuses_other_heads():
         RingCache4(heads=2, head_dim=64, grid_h=2, grid_w=5)
     with pytest.raises(ops.PrepError, match="heads"):
         RingCache4(heads=2, grid_h=2, grid_w=5, pool=Kv4Pool(4, 3))
+
+
+# ---------------------------------------------------------------------------------------
+# The workspace of the tiles kernel
+# ---------------------------------------------------------------------------------------
+def test_tiles_workspace_has_room_from_any_16_byte_boundary(lib):
+    """A query row's partial results (128 sums, a reference and a sum of weights) for 256 rows of the first and
+    the last unit of each CTA, 16 bytes for each unit, all behind the first 32-byte boundary: the kernel stores 32
+    bytes at a time.  1,000 steps are more than the grid of 148 CTAs needs."""
+    args = attn(cache(table_pages=1000, num_pages=5000), kv_tokens=16000, kernel=_lib.KV4_TILES)
+    need = ctypes.c_int64(0)
+    assert lib.ps_kv4_attention_workspace(ctypes.byref(args), ctypes.byref(need)) == _lib.OK
+    assert need.value == 2 * 148 * 256 * (128 * 4 + 8) + 2 * 4 * 16 + 16
+    for offset in (0, 16):
+        args.workspace, args.workspace_bytes = BASE + offset, need.value - 1
+        assert lib.ps_attention_kv4(ctypes.byref(args), None) == _lib.ERR_NULL
+    args.workspace, args.workspace_bytes = BASE + 8, need.value
+    assert lib.ps_attention_kv4(ctypes.byref(args), None) == _lib.ERR_ALIGN
