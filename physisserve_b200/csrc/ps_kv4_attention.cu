@@ -677,9 +677,11 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const __grid_constant_
 //                overwrites the S columns that were read; P V starts on the first half of the keys while
 //                the second half is exponentiated.  Warp 12 owns the tensor memory (512 columns:
 //                O0 | S0 | O1 | S1).
+//   warp 15      writes which CTAs share each unit, for the merge.
 // tcgen05.mma operations of one thread complete in issue order, so a commit after S_i(t+1) also reports
 // P_i(t) V(t) done.  All waits are bounded: one that runs out raises the CTA's abort flag, every role
-// leaves its loop, the issuers wait for their MMAs and the tensor memory is freed.
+// leaves its loop, the issuers wait for their MMAs and the tensor memory is freed; the rows' values are
+// undefined then, the units' table is not.
 constexpr int kM = 128;
 constexpr int kUnitRows = 2 * kM;
 constexpr int kTile16 = kM * kKv4D * 2;    // bytes of a 128 x 128 fp16 tile
@@ -1120,6 +1122,14 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
         }
       }
       tc_commit(bar(kMmaDone));
+    } else if (warp == 15 && lane == 0) {
+      // The units that begin here and the CTAs that share each, for the merge.  Nothing is waited for: the merge
+      // runs after a CTA that gave up too, and what it takes indices from has to be there all the same.
+      for (bool more = w.begin(p, start, n_steps); more; more = w.next(p)) {
+        if (w.j0 != 0) continue;
+        const int last = static_cast<int>((per * blockIdx.x + w.done + w.steps - 1) / per);
+        p.ws_units[w.unit(p)] = make_int4(static_cast<int>(blockIdx.x), last, w.first() ? 0 : 1, 0);
+      }
     }
     __syncwarp();
   } else {
@@ -1330,10 +1340,6 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
                          : "memory");
         }
         p.ws_ml[slot] = make_float2(m, l);
-      }
-      if (qi == 0 && row == 0 && w.j0 == 0) {
-        const int last = static_cast<int>((per * blockIdx.x + w.done + w.steps - 1) / per);
-        p.ws_units[w.unit(p)] = make_int4(static_cast<int>(blockIdx.x), last, w.first() ? 0 : 1, 0);
       }
       tc_fence_before();
     }

@@ -867,3 +867,37 @@ def test_attention_workspace_on_any_16_byte_boundary(kernel, offset):
     check_attention(got, q, k, v, [rows], 2)
     assert bool((arena[:offset] == 0x5a).all()) and bool((arena[offset + need:] == 0x5a).all())
     assert not bool((workspace == 0x5a).all())
+
+
+@pytest.mark.parametrize("members,Lq,heads,rows,cb,lens", [
+    (1, 3, 1, 1, 0, None),                              # one unit, one step
+    (1, 300, 2, 2500, 0, None),                         # units shared by several CTAs
+    (3, 700, 4, 900, 70, [900, 0, 333]),                # unlike units, more of them than CTAs have segments
+    (2, 5000, 40, 130, 1, [130, 64]),                   # many units a CTA
+])
+def test_the_tiles_kernel_leaves_every_unit_its_ctas(members, Lq, heads, rows, cb, lens):
+    """The merge takes indices from the units' table, so every entry has to be there: the first CTA, the last one
+    and the first one's slot of each (member, head, 256 query rows), by the same cut of all steps into ranges."""
+    pages, table, k, v = fill(members, rows, heads, 64, 63)
+    q = torch.randn(members, Lq, heads * 128, generator=gen(64)).bfloat16()
+    dev = q.to(DEV), pages.to(DEV), table.to(DEV)
+    n = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=DEV)
+    need = workspace_bytes(*dev, rows, heads, _lib.KV4_TILES, 0 if n is None else n.data_ptr())
+    workspace = torch.full((need,), 0xff, dtype=torch.uint8, device=DEV)
+    assert workspace.data_ptr() % 32 == 0
+    ops.attention_kv4(*dev, rows if n is None else n, heads=heads, causal_block=cb, max_kv_tokens=rows, kernel="tiles",
+                      workspace=workspace)
+    steps = []
+    for b in range(members):
+        limits = kv4.limits(rows if lens is None else lens[b], Lq, cb)
+        last = [min(Lq, 256 * (i + 1)) - 1 for i in range(-(-Lq // 256))]
+        steps += [max(1, -(-int(limits[i]) // 128)) for i in last] * heads
+    steps = torch.tensor(steps)
+    before = steps.cumsum(0) - steps
+    most = len(steps) * max(1, -(-rows // 128))
+    grid = min(torch.cuda.get_device_properties(0).multi_processor_count, -(-most // 2))
+    per = max(-(-int(steps.sum()) // grid), 2)
+    want = torch.stack([before // per, (before + steps - 1) // per, (before % per != 0).long(), torch.zeros_like(steps)], 1)
+    at = 2 * grid * 256 * (128 * 4 + 8)
+    got = workspace[at:at + 16 * len(steps)].view(torch.int32).view(-1, 4).cpu()
+    assert torch.equal(got.long(), want)
