@@ -288,6 +288,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
     // ------------------------------- producer -------------------------------
     int t = 0;
     if (lane < R) sh.lim[lane] = token_limit(p, n, min(row0 + lane, p.rows - 1) / p.group);
+    __syncwarp();  // the consumers learn of all of them by lane 0's arrival below
     // Lane i: table entry of the tile's page i, a tile ahead (unconditional loads, so that nothing waits for
     // them before they are used).
     auto seen = [&](int j) { return lane < segs && j * kTileKeys + (lane << shift) < lim_top; };

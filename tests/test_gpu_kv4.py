@@ -901,3 +901,20 @@ def test_the_tiles_kernel_leaves_every_unit_its_ctas(members, Lq, heads, rows, c
     at = 2 * grid * 256 * (128 * 4 + 8)
     got = workspace[at:at + 16 * len(steps)].view(torch.int32).view(-1, 4).cpu()
     assert torch.equal(got.long(), want)
+
+
+@pytest.mark.parametrize("page_rows", [16, 128])
+@pytest.mark.parametrize("rows", [131, 200])
+def test_attention_limits_of_rows_whose_first_pages_are_missing(rows, page_rows):
+    """Eight rows of unlike limits over a window whose first tile has no page: nothing but the limits themselves
+    tells the warps what each row sees."""
+    pages, table, k, v = fill(3, rows, 2, page_rows, 66)
+    table[:, :128 // page_rows] = -1
+    absent = torch.zeros(3, rows, dtype=torch.bool)
+    absent[:, :128] = True
+    q = torch.randn(3, 8, 2 * 128, generator=gen(67)).bfloat16()
+    ops.kv4_counters()
+    for _ in range(5):
+        got = ops.attention_kv4(q.to(DEV), pages.to(DEV), table.to(DEV), rows, heads=2, causal_block=1, kernel="rows")
+        check_attention(got, q, k, v, [rows] * 3, 2, 1, absent=absent)
+    assert ops.kv4_counters().bad_pages > 0
