@@ -152,8 +152,8 @@ PS_API int32_t ps_kv4_read_validate(const ps_kv4_read_args* args);
 /* Softmax attention of every query row over the window rows it sees.  Q and the
  * dequantised K and V enter the products in fp16: code * scale has six
  * significant bits, so K and V are exact, and a query row is scaled by the power
- * of two that brings its largest element to [1, 2), so that nothing of it that
- * matters at 24 bits is lost (the tensor scales and that power are applied to the
+ * of two that brings its largest element to [1, 2) ([2, 4) from 2^127 on), so
+ * that nothing of it that matters at 24 bits is lost (the tensor scales and that power are applied to the
  * scores in fp32).  Scores, softmax statistics and sums are fp32; probabilities
  * are rounded to fp16 for P V; the output is rounded once to bf16. */
 PS_API int32_t ps_attention_kv4(const ps_kv4_attn_args* args, void* stream);

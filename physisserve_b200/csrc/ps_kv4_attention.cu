@@ -66,13 +66,15 @@ __device__ __forceinline__ int token_limit(const AParams& p, int n, int t) {
 }
 
 // Power of two that brings a row's largest magnitude `top` (>= 0) into [1, 2), and its inverse; 1 for
-// zero, subnormal and non-finite rows.
+// zero, subnormal and non-finite rows.  The inverse of 2^127 is subnormal: rows from there on come into
+// [2, 4), which fp16 holds with the same bits.
 __device__ __forceinline__ float row_power(float top, float& back) {
-  const uint32_t e = __float_as_uint(top) >> 23;
-  if (e < 2 || e > 252) {
+  uint32_t e = __float_as_uint(top) >> 23;
+  if (e < 2 || e > 254) {
     back = 1.f;
     return 1.f;
   }
+  e = min(e, 253u);
   back = __uint_as_float(e << 23);
   return __uint_as_float((254u - e) << 23);
 }

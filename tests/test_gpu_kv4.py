@@ -918,3 +918,17 @@ def test_attention_limits_of_rows_whose_first_pages_are_missing(rows, page_rows)
         got = ops.attention_kv4(q.to(DEV), pages.to(DEV), table.to(DEV), rows, heads=2, causal_block=1, kernel="rows")
         check_attention(got, q, k, v, [rows] * 3, 2, 1, absent=absent)
     assert ops.kv4_counters().bad_pages > 0
+
+
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
+@pytest.mark.parametrize("Lq", [2, 140])
+@pytest.mark.parametrize("exponent", [124, 125, 126, 127])
+def test_attention_query_rows_up_to_the_largest_numbers(exponent, Lq, kernel):
+    """Largest elements in [2^exponent, 2^(exponent + 1)): finite in bf16, so the rows' outputs are."""
+    pages, table, k, v = fill(1, 200, 2, 16, 40, k_scale=0.02, k_size=0.02)
+    q = (torch.rand(1, Lq, 2 * 128, generator=gen(41)) * 2 - 1).bfloat16() * 1.5 * 2.0 ** exponent
+    q[..., ::128] = 1.75 * 2.0 ** exponent
+    assert q.dtype == torch.bfloat16 and bool(torch.isfinite(q).all())
+    scale = 2.0 ** (3 - exponent)
+    got = ops.attention_kv4(q.to(DEV), pages.to(DEV), table.to(DEV), 200, heads=2, scale=scale, k_scale=0.02, kernel=kernel)
+    check_attention(got, q, k, v, [200], 2, scale=scale)
