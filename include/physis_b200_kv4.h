@@ -153,9 +153,11 @@ PS_API int32_t ps_kv4_read_validate(const ps_kv4_read_args* args);
  * dequantised K and V enter the products in fp16: code * scale has six
  * significant bits, so K and V are exact, and a query row is scaled by the power
  * of two that brings its largest element to [1, 2) ([2, 4) from 2^127 on), so
- * that nothing of it that matters at 24 bits is lost (the tensor scales and that power are applied to the
- * scores in fp32).  Scores, softmax statistics and sums are fp32; probabilities
- * are rounded to fp16 for P V; the output is rounded once to bf16. */
+ * that nothing of it that matters at 24 bits is lost (the tensor scales and that
+ * power are applied to the scores in fp32).  Scores, softmax statistics and sums
+ * are fp32; probabilities are rounded to fp16 for P V, with an absolute error of
+ * 2^-32 of the row's largest at most where that is more than 2^-11 of their own;
+ * the output is rounded once to bf16. */
 PS_API int32_t ps_attention_kv4(const ps_kv4_attn_args* args, void* stream);
 PS_API int32_t ps_kv4_attention_validate(const ps_kv4_attn_args* args);
 /* Bytes of scratch that ps_attention_kv4 needs for these arguments on the current device (of the pointers

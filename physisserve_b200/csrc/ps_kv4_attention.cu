@@ -65,6 +65,12 @@ __device__ __forceinline__ int token_limit(const AParams& p, int n, int t) {
   return lim < 0 ? 0 : (lim > n ? n : static_cast<int>(lim));
 }
 
+// Probabilities are taken against a reference of their row that lags the running maximum by up to kLag (log2
+// units), so that it seldom moves, and 2^kLift times larger, so that fp16 holds them from 2^15 (its largest
+// power of two) down to 2^-24: what is lost of one is at most 2^-32 of the largest probability.  Without the
+// lift keys below 2^-25 of it were dropped from P V but not from the sum, all of them together.
+constexpr float kLag = 8.f, kLift = 7.f;
+
 // Power of two that brings a row's largest magnitude `top` (>= 0) into [1, 2), and its inverse; 1 for
 // zero, subnormal and non-finite rows.  The inverse of 2^127 is subnormal: rows from there on come into
 // [2, 4), which fp16 holds with the same bits.
@@ -437,9 +443,8 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) grow |= acc[u][e] > m[e & 1] + 8.f;
-      // The reference of a row moves only when a score exceeds it by more than 8 (probabilities are
-      // exact for any reference; fp16 holds them up to 2^8 with the same relative rounding).
+        for (int e = 0; e < 4; ++e) grow |= acc[u][e] > m[e & 1] + kLag;
+      // The reference of a row moves only when a score exceeds it by more than kLag.
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -462,7 +467,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
       }
       uint32_t pb[U][2];
       {
-        const float r0 = m[0] == -INFINITY ? 0.f : m[0], r1 = m[1] == -INFINITY ? 0.f : m[1];
+        const float r0 = m[0] == -INFINITY ? 0.f : m[0] - kLift, r1 = m[1] == -INFINITY ? 0.f : m[1] - kLift;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const float p0 = fast_exp2(acc[u][0] - r0), p1 = fast_exp2(acc[u][1] - r1);
@@ -1242,8 +1247,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
           largest(xb);
         }
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
-        // The reference moves only when a score exceeds it by more than 8: P is exact for any reference.
-        const bool grow = top > m + 8.f;
+        // The reference moves only when a score exceeds it by more than kLag.
+        const bool grow = top > m + kLag;
         const float alpha = grow ? fast_exp2(m - top) : 1.f;
         if (grow) {
           l *= alpha;
@@ -1261,7 +1266,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
             tmem_st16(o_addr + 16 * c, o);
           }
         }
-        const float ref = m == -INFINITY ? 0.f : m;
+        const float ref = m == -INFINITY ? 0.f : m - kLift;
         const f32x2 scale2 = f2_make(scale, scale), ref2 = f2_make(-ref, -ref);
         f32x2 sum[2] = {0, 0};
         // Tile 0's k-th turn follows tile 1's (k-1)-th, tile 1's k-th follows tile 0's k-th.

@@ -932,3 +932,32 @@ def test_attention_query_rows_up_to_the_largest_numbers(exponent, Lq, kernel):
     scale = 2.0 ** (3 - exponent)
     got = ops.attention_kv4(q.to(DEV), pages.to(DEV), table.to(DEV), 200, heads=2, scale=scale, k_scale=0.02, kernel=kernel)
     check_attention(got, q, k, v, [200], 2, scale=scale)
+
+
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
+@pytest.mark.parametrize("Lq", [4, 200])
+def test_attention_small_probabilities_count(Lq, kernel):
+    """Every 32nd key takes nearly all of the probability and has a V of zero: what the output holds comes from
+    keys of 2^-21.6 to 2^-26 of it.  Bound: the output's rounding 2^-8 |out|, the probabilities' 2^-11 and the
+    scores' and exponentials' 2^-13 of A = out, and for probabilities below fp16's normal range half of its last
+    step, 2^-25, 2^7 times smaller against the largest: N 2^-32 max|v| / sum."""
+    rows = 1000
+    n, table = make_table(1, -(-rows // 32), 2, 50)
+    pages = torch.full((n, 1, 2, 32 * 72), 0xff, dtype=torch.uint8)
+    top = torch.arange(rows) % 32 == 0
+    x = torch.zeros(rows, 1, 128)
+    x[top, 0, 0] = 6.0
+    y = torch.rand(rows, 1, 128, generator=gen(51)) + 0.5
+    y[top] = 0.0
+    for which, t in ((0, x), (1, y)):
+        kv4.store(pages, table, torch.arange(rows), t, which, 1.0)
+    k, v = (kv4.load(pages, table, torch.arange(rows), w, 1.0)[None] for w in (0, 1))
+    assert torch.equal(k[0].float(), x)
+    q = torch.zeros(1, Lq, 128, dtype=torch.bfloat16)
+    q[0, :, 0] = torch.tensor([2.5, 2.75, 2.84375, 3.0]).repeat(-(-Lq // 4))[:Lq]    # times 6 / ln 2: 21.6, 23.8, 24.6, 26.0
+    got = ops.attention_kv4(q.to(DEV), pages.to(DEV), table.to(DEV), rows, heads=1, scale=1.0, key_chunks=1, kernel=kernel)
+    want, size = kv4.attention(q, k, v, [rows], 1, scale=1.0)
+    bound = 2 ** -8 * want + 2 ** -10 * size + 2 ** -32 * rows * float(v.max()) / int(top.sum())
+    assert float(want.min()) > 2 ** -24
+    err = (got.cpu().double().view(want.shape) - want).abs()
+    assert bool((err <= bound).all()), f"{float((err / bound).max()):.2f} x the bound"
