@@ -164,8 +164,17 @@ PS_API int32_t ps_kv4_attention_validate(const ps_kv4_attn_args* args);
  * only kv_lens matters: whether it is NULL). */
 PS_API int32_t ps_kv4_attention_workspace(const ps_kv4_attn_args* args, int64_t* bytes);
 
-/* Counts on the current device since the last reset: counts[0] accesses to pages
- * outside the pool, counts[1] blocks that held an infinity or a NaN, counts[2]
+/* What ps_kv4_counters clears after reading (any other value clears every count). */
+typedef enum ps_kv4_reset {
+  PS_KV4_KEEP = 0,
+  PS_KV4_RESET = 1,          /* every count */
+  PS_KV4_RESET_TIMEOUTS = 2  /* counts[2] alone */
+} ps_kv4_reset;
+
+/* Counts on the current device since each was last cleared: counts[0] pages outside
+ * the pool that calls came upon (an append counts each token of such a page, a read
+ * each 16 elements of a row and head, an attention each thread block that takes
+ * its keys), counts[1] blocks that held an infinity or a NaN, counts[2]
  * bounded waits that ran out (the outputs of that call are undefined).
  * Synchronises the device first. */
 PS_API int32_t ps_kv4_counters(uint32_t counts[3], int32_t reset);

@@ -35,6 +35,8 @@ LAUNCH_STREAM, LAUNCH_PDL, LAUNCH_PDL_EARLY_INPUTS = 0, 1, 2
 SEQ_PREP, SEQ_SINK = 0, 1
 # ps_kv4_kernel
 KV4_AUTO, KV4_ROWS, KV4_TILES = 0, 1, 2
+# ps_kv4_reset
+KV4_KEEP, KV4_RESET, KV4_RESET_TIMEOUTS = 0, 1, 2
 # PS_KV4_ROW_BYTES
 KV4_ROW_BYTES = 72
 # PS_ATTN_STATIC_SCRATCH_BYTES (include/physis_b200_attention.h)

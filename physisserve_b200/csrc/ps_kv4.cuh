@@ -13,21 +13,22 @@ constexpr int kKv4D = PS_KV4_HEAD_DIM;
 constexpr int kKv4Row = PS_KV4_ROW_BYTES;
 
 // Counters of the translation unit that includes this header (ps_kv4_counters adds them up).
-enum { kKv4BadPages, kKv4NonFinite, kKv4Timeouts, kKv4Counters };
+enum { kKv4BadPages, kKv4NonFinite, kKv4Timeouts, kKv4Counters };  // the timeouts last
 static __device__ unsigned int g_kv4_counts[kKv4Counters];
 
-// Adds this translation unit's counts to `counts` and clears them if `reset`.
-static inline cudaError_t kv4_take_counts(uint32_t* counts, bool reset) {
+// Adds this translation unit's counts to `counts` and clears those that `reset` (ps_kv4_reset) names.
+static inline cudaError_t kv4_take_counts(uint32_t* counts, int reset) {
   uint32_t own[kKv4Counters] = {};
   cudaError_t err = cudaMemcpyFromSymbol(own, g_kv4_counts, sizeof(own));
   for (int i = 0; i < kKv4Counters; ++i) counts[i] += own[i];
-  if (err == cudaSuccess && reset) {
+  if (err == cudaSuccess && reset != PS_KV4_KEEP) {
+    const int first = reset == PS_KV4_RESET_TIMEOUTS ? kKv4Timeouts : 0;
     memset(own, 0, sizeof(own));
-    err = cudaMemcpyToSymbol(g_kv4_counts, own, sizeof(own));
+    err = cudaMemcpyToSymbol(g_kv4_counts, own, (kKv4Counters - first) * sizeof(own[0]), first * sizeof(own[0]));
   }
   return err;
 }
-cudaError_t kv4_attention_counts(uint32_t* counts, bool reset);  // ps_kv4_attention.cu
+cudaError_t kv4_attention_counts(uint32_t* counts, int reset);  // ps_kv4_attention.cu
 
 // A cache as kernels see it.
 struct Kv4Dev {

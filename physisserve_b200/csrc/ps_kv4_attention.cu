@@ -1591,7 +1591,7 @@ static cudaError_t launch(void (*fn)(A...), int64_t blocks, int threads, int sme
 
 }  // namespace
 
-cudaError_t kv4_attention_counts(uint32_t* counts, bool reset) { return kv4_take_counts(counts, reset); }
+cudaError_t kv4_attention_counts(uint32_t* counts, int reset) { return kv4_take_counts(counts, reset); }
 
 }  // namespace ps
 

@@ -846,8 +846,8 @@ extern "C" int32_t ps_kv4_counters(uint32_t* counts, int32_t reset) {
   if (!counts) return ps::fail(PS_ERR_NULL, "counts is NULL");
   counts[0] = counts[1] = counts[2] = 0;
   cudaError_t err = cudaDeviceSynchronize();
-  if (err == cudaSuccess) err = ps::kv4_take_counts(counts, reset != 0);
-  if (err == cudaSuccess) err = ps::kv4_attention_counts(counts, reset != 0);
+  if (err == cudaSuccess) err = ps::kv4_take_counts(counts, reset);
+  if (err == cudaSuccess) err = ps::kv4_attention_counts(counts, reset);
   if (err != cudaSuccess) return ps::fail(PS_ERR_LAUNCH, "reading the cache counters: %s", cudaGetErrorString(err));
   return PS_OK;
 }

@@ -1031,7 +1031,8 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, kv_
                              workspace.numel() * workspace.element_size())
         _check(lib.ps_attention_kv4(args, _current_stream(device_index)))
     if check_timeouts:
-        count = kv4_counters(reset=True, device=device_index).timeouts
+        # The other counts stay for who asks for them.
+        count = _kv4_counts(_lib.KV4_RESET_TIMEOUTS, device_index).timeouts
         if count:
             raise PrepError(f"{count} bounded wait(s) of the attention kernel ran out on cuda:{device_index}: "
                             "the outputs of the calls since the last check are undefined")
@@ -1046,15 +1047,21 @@ class Kv4Counters(NamedTuple):
     timeouts: int
 
 
-def kv4_counters(reset: bool = True, device: int | None = None) -> Kv4Counters:
-    """Counts of the 4-bit cache's kernels on ``device`` since the last reset (synchronises it): accesses to
-    pages outside the pool, blocks of 16 elements that held an infinity or a NaN when they were stored, and
-    bounded waits that ran out (the outputs of the calls since are then undefined)."""
-    index = torch.cuda.current_device() if device is None else int(device)
+def _kv4_counts(reset: int, index: int) -> Kv4Counters:
     counts = (ctypes.c_uint32 * 3)()
     with _on_device(index):
-        _check(_lib.load().ps_kv4_counters(counts, int(reset)))
+        _check(_lib.load().ps_kv4_counters(counts, reset))
     return Kv4Counters(*(int(c) for c in counts))
+
+
+def kv4_counters(reset: bool = True, device: int | None = None) -> Kv4Counters:
+    """Counts of the 4-bit cache's kernels on ``device`` since the last reset (synchronises it): pages outside
+    the pool that calls came upon (an append counts each token of such a page, a read each 16 elements of a row
+    and head, an attention each thread block that takes its keys), blocks of 16 elements that held an infinity
+    or a NaN when they were stored, and bounded waits that ran out (the outputs of the calls since are
+    then undefined; ``attention_kv4(check_timeouts=True)`` takes these, and only these)."""
+    return _kv4_counts(_lib.KV4_RESET if reset else _lib.KV4_KEEP,
+                       torch.cuda.current_device() if device is None else int(device))
 
 
 def wait_selftest(limit_us: int = 20000, device: int | None = None) -> None:

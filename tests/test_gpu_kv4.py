@@ -961,3 +961,18 @@ def test_attention_small_probabilities_count(Lq, kernel):
     assert float(want.min()) > 2 ** -24
     err = (got.cpu().double().view(want.shape) - want).abs()
     assert bool((err <= bound).all()), f"{float((err / bound).max()):.2f} x the bound"
+
+
+def test_looking_for_timeouts_keeps_the_other_counts():
+    kwargs, _, _, _ = append_case(1, 4, 4, 1, 2, 2, 16, torch.bfloat16, 1, seed=8)
+    kwargs["v"][3, 5] = float("nan")
+    table = kwargs["table"].clone()
+    ops.kv4_counters()
+    ops.qk_norm_rope_kv4(**kwargs)
+    kwargs["table"][0, 0] = -1
+    ops.read_kv4(kwargs["pages"], kwargs["table"], 16)
+    q = torch.randn(1, 1, 256, generator=gen(60)).bfloat16().to(DEV)
+    ops.attention_kv4(q, kwargs["pages"], table, 16, heads=2, check_timeouts=True)
+    counts = ops.kv4_counters(reset=False)
+    assert counts.nonfinite == 1 and counts.bad_pages > 0 and counts.timeouts == 0
+    assert ops.kv4_counters() == counts and ops.kv4_counters() == (0, 0, 0)
