@@ -251,8 +251,9 @@ __global__ void __launch_bounds__(NB == 5 ? 256 : kMaxTpt, NB == 5 ? 2 : 1) kv4_
   // Positions and the cache row.
   const int f = static_cast<int>(div_by(static_cast<uint32_t>(l), sq.hw_magic));
   const int rr = l - f * sq.hw;
-  int ring = sq.ring_slot0 + f;
-  if (ring >= sq.ring_frames) ring -= sq.ring_frames;
+  // (unsigned: a ring of one-token frames may have more than 2^30 of them)
+  uint32_t ring = static_cast<uint32_t>(sq.ring_slot0) + static_cast<uint32_t>(f);
+  if (ring >= static_cast<uint32_t>(sq.ring_frames)) ring -= static_cast<uint32_t>(sq.ring_frames);
   const int64_t kv_row = sq.ring_row + static_cast<int64_t>(ring) * sq.hw + rr;
   const int64_t page = active && (do_k || do_v) ? kv4_page(p.cache, kv_row >> p.cache.shift, lt == 0) : -1;
   // The token's K row of this thread's first head; V's is `half` bytes further, the next head's `step`.

@@ -976,3 +976,20 @@ def test_looking_for_timeouts_keeps_the_other_counts():
     counts = ops.kv4_counters(reset=False)
     assert counts.nonfinite == 1 and counts.bad_pages > 0 and counts.timeouts == 0
     assert ops.kv4_counters() == counts and ops.kv4_counters() == (0, 0, 0)
+
+
+def test_append_to_a_ring_of_nearly_two_to_the_31_frames():
+    """One-token frames around the end of the largest ring: the slot of the frame behind the last one is 0, by
+    arithmetic that passes 2^31."""
+    frames, page_rows, heads = (1 << 31) - 1, 128, 2
+    table = torch.full((1, (1 << 31) // page_rows), -1, dtype=torch.int32, device=DEV)
+    table[0, 0], table[0, -1] = 2, 1
+    pages = ops.kv4_pages(3, heads, page_rows, DEV)
+    x = torch.randn(5, heads * 128, generator=gen(70)).bfloat16()
+    ops.kv4_counters()
+    ops.qk_norm_rope_kv4(heads=heads, seqs=[ops.Seq(0, 5, 1, 1, 0, 0, 0, frames, frames - 2)], v=x.to(DEV), pages=pages, table=table)
+    assert ops.kv4_counters() == (0, 0, 0)
+    want = torch.zeros_like(pages, device="cpu")
+    at = torch.cat([torch.tensor([1, 1]) * page_rows + torch.tensor([125, 126]), 2 * page_rows + torch.arange(3)])
+    kv4.store(want, torch.arange(3)[None], at, x.view(5, heads, 128), 1, 1.0)
+    assert torch.equal(pages.cpu(), want)
