@@ -1458,6 +1458,8 @@ static int build_attn(const ps_kv4_attn_args* a, APlan* plan, bool host_only) {
   const int hk = a->cache.kv_heads;
   if (a->heads < 1 || a->heads % hk)
     return fail(PS_ERR_SHAPE, "heads=%d is not a multiple of kv_heads=%d", a->heads, hk);
+  // The kernels take the columns of a token in 32 bits.
+  if (a->heads > INT32_MAX / kKv4D) return fail(PS_ERR_UNSUPPORTED, "heads=%d: columns beyond 2^31", a->heads);
   if (a->q_tokens < 0 || a->kv_tokens < 0 || a->causal_block < 0)
     return fail(PS_ERR_SHAPE, "q_tokens=%d kv_tokens=%d causal_block=%d", a->q_tokens, a->kv_tokens, a->causal_block);
   if (a->kv_tokens > a->cache.table_pages * a->cache.page_rows)

@@ -305,3 +305,10 @@ def test_tiles_workspace_has_room_from_any_16_byte_boundary(lib):
         assert lib.ps_attention_kv4(ctypes.byref(args), None) == _lib.ERR_NULL
     args.workspace, args.workspace_bytes = BASE + 8, need.value
     assert lib.ps_attention_kv4(ctypes.byref(args), None) == _lib.ERR_ALIGN
+
+
+def test_attention_refuses_columns_beyond_32_bits(lib):
+    for heads, want in (((1 << 24) - 4, _lib.OK), (1 << 24, _lib.ERR_UNSUPPORTED)):
+        wide = attn(heads=heads, q_tokens=1, q_row_stride=heads * 128, q_member_stride=heads * 128, out_row_stride=heads * 128,
+                    out_member_stride=heads * 128)
+        assert lib.ps_kv4_attention_validate(ctypes.byref(wide)) == want, lib.ps_error_message()
