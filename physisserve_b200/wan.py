@@ -349,9 +349,12 @@ def prep_ring(q, k, v, q_weight, k_weight, eps, freqs_cos, freqs_sin, cache: Rin
     ring row block b of ``cache.k``/``cache.v``); positions[b]: its ``RingPositions``.
     Writes rotated K and V into each member's slot (sink region for chunk 0, also saving
     the pre-RoPE sink K), re-rotates relocated sinks, and returns rotated Q [batch, L, C].
-    A ``RingCache4`` takes the pages that the members' windows reach first.
+    A ``RingCache4`` takes the pages that the members' windows reach first.  ``heads_per_thread`` overrides
+    the work split of the ring's kernel (0 = automatic); the 4-bit cache's has no such choice.
     """
     B, L, C = q.shape
+    if heads_per_thread and isinstance(cache, RingCache4):
+        raise PrepError(f"heads_per_thread={heads_per_thread}: only the ring's kernel has this choice")
     if len(positions) != B or cache.batch != B:
         raise PrepError(f"{len(positions)} positions / cache batch {cache.batch} for {B} members")
     hw = cache.tokens_per_frame

@@ -312,3 +312,15 @@ def test_attention_refuses_columns_beyond_32_bits(lib):
         wide = attn(heads=heads, q_tokens=1, q_row_stride=heads * 128, q_member_stride=heads * 128, out_row_stride=heads * 128,
                     out_member_stride=heads * 128)
         assert lib.ps_kv4_attention_validate(ctypes.byref(wide)) == want, lib.ps_error_message()
+
+
+def test_prep_ring_refuses_a_split_that_the_4_bit_cache_does_not_have():
+    from physisserve_b200.wan import RingCache4, prep_ring, wan_rope_tables, window_layout
+
+    cache = RingCache4(heads=1, grid_h=2, grid_w=2, capacity=2, sink_frames=1)
+    x, w = torch.zeros(1, 4, 128, dtype=torch.bfloat16), torch.ones(128, dtype=torch.bfloat16)
+    pos = [window_layout(0, first_frames=1)]
+    free = cache.pool.free_pages
+    with pytest.raises(ops.PrepError, match="heads_per_thread"):
+        prep_ring(x, x, x, w, w, 1e-6, *wan_rope_tables(128, 8), cache, pos, heads_per_thread=2)
+    assert cache.pool.free_pages == free
