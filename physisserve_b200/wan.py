@@ -21,6 +21,7 @@ rotated rows.
 """
 from __future__ import annotations
 
+import threading
 from dataclasses import dataclass
 from typing import Sequence
 
@@ -225,13 +226,15 @@ class RingCache:
 
 class Kv4Pool:
     """Pages of 4-bit K/V rows (``ops.kv4_pages``) shared by the ``RingCache4`` of many cells: a cell holds
-    the pages that its window has reached and gives them back when its stream ends."""
+    the pages that its window has reached and gives them back when its stream ends.  Cells of several host
+    threads may share a pool (a cell itself belongs to one)."""
 
     def __init__(self, num_pages: int, heads: int, page_rows: int = 128, device=None):
         self.pages = kv4_pages(num_pages, heads, page_rows, device)
         self.page_rows = page_rows
         self._free = list(range(num_pages - 1, -1, -1))
         self._taken: set[int] = set()
+        self._lock = threading.Lock()
 
     @property
     def free_pages(self) -> int:
@@ -239,21 +242,23 @@ class Kv4Pool:
 
     def take(self, count: int) -> list[int]:
         """``count`` free pages."""
-        if count > len(self._free):
-            raise PrepError(f"the pool has {len(self._free)} free pages, {count} are needed")
-        taken = self._free[len(self._free) - count:]
-        del self._free[len(self._free) - count:]
-        self._taken.update(taken)
+        with self._lock:
+            if count > len(self._free):
+                raise PrepError(f"the pool has {len(self._free)} free pages, {count} are needed")
+            taken = self._free[len(self._free) - count:]
+            del self._free[len(self._free) - count:]
+            self._taken.update(taken)
         return taken[::-1]
 
     def give(self, pages: Sequence[int]) -> None:
         """Takes pages back.  Work on them that is still running on another stream than the one their
         next holder uses must be waited for first."""
         given = set(pages)
-        if len(given) != len(pages) or not given <= self._taken:
-            raise PrepError(f"pages {list(pages)} are not all held by someone, each once")
-        self._taken -= given
-        self._free.extend(reversed(pages))
+        with self._lock:
+            if len(given) != len(pages) or not given <= self._taken:
+                raise PrepError(f"pages {list(pages)} are not all held by someone, each once")
+            self._taken -= given
+            self._free.extend(reversed(pages))
 
 
 class RingCache4:
@@ -306,17 +311,20 @@ class RingCache4:
         """Takes the pages that member b's first ``rows[b]`` rows still need (outside of a captured graph: the
         new table entries are copied from the host; a graph's windows are reserved ahead of it)."""
         need = [-(-n // self.pool.page_rows) - len(held) for n, held in zip(rows, self._held)]
-        if sum(n for n in need if n > 0) > self.pool.free_pages:
-            raise PrepError(f"the pool has {self.pool.free_pages} free pages, {sum(n for n in need if n > 0)} are needed")
-        for b, n in enumerate(need):
-            if n > 0:
-                new, at = self.pool.take(n), len(self._held[b])
-                try:
-                    self.table[b, at:at + n] = torch.tensor(new, dtype=torch.int32)
-                except RuntimeError:  # a copy from the host fails in a captured graph
-                    self.pool.give(new)
-                    raise
-                self._held[b] += new
+        count = sum(n for n in need if n > 0)
+        if count == 0:
+            return
+        new, at = self.pool.take(count), 0
+        try:
+            for b, n in enumerate(need):
+                if n > 0:
+                    own, held = new[at:at + n], self._held[b]
+                    self.table[b, len(held):len(held) + n] = torch.tensor(own, dtype=torch.int32)
+                    held += own
+                    at += n
+        except RuntimeError:  # a copy from the host fails in a captured graph
+            self.pool.give(new[at:])
+            raise
 
     def release(self) -> None:
         """Gives every page back; the cache starts over with chunk 0."""

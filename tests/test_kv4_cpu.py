@@ -324,3 +324,48 @@ def test_prep_ring_refuses_a_split_that_the_4_bit_cache_does_not_have():
     with pytest.raises(ops.PrepError, match="heads_per_thread"):
         prep_ring(x, x, x, w, w, 1e-6, *wan_rope_tables(128, 8), cache, pos, heads_per_thread=2)
     assert cache.pool.free_pages == free
+
+
+def test_pool_gives_two_threads_different_pages():
+    """A thread asks for pages while another is in the middle of taking its own."""
+    import threading
+
+    from physisserve_b200.wan import Kv4Pool
+
+    pool, other = Kv4Pool(8, 1, page_rows=16), []
+    thread = threading.Thread(target=lambda: other.extend(pool.take(3)))
+
+    class Interrupted(list):
+        def __getitem__(self, at):
+            if not thread.ident:
+                thread.start()
+                thread.join(0.3)
+            return list.__getitem__(self, at)
+
+        def __delitem__(self, at):
+            if not thread.ident:
+                thread.start()
+                thread.join(0.3)
+            list.__delitem__(self, at)
+
+    pool._free = Interrupted(pool._free)
+    mine = pool.take(3)
+    thread.join()
+    assert len(set(mine) | set(other)) == 6 and sorted(mine + other + pool.take(2)) == list(range(8))
+
+
+def test_a_reservation_is_taken_whole_or_not_at_all():
+    """Pages that another thread takes between a cache's look at the pool and its taking."""
+    from physisserve_b200.wan import Kv4Pool, RingCache4
+
+    class Raced(Kv4Pool):
+        def take(self, count):
+            if not self._taken:
+                Kv4Pool.take(self, 5)
+            return Kv4Pool.take(self, count)
+
+    pool = Raced(8, 1, page_rows=16)
+    cell = RingCache4(heads=1, grid_h=2, grid_w=4, capacity=4, sink_frames=2, batch=2, pool=pool)
+    with pytest.raises(ops.PrepError, match="free pages"):
+        cell.reserve([40, 17])
+    assert pool.free_pages == 3 and bool((cell.table == -1).all()) and cell._held == [[], []]
