@@ -30,6 +30,15 @@ static inline cudaError_t kv4_take_counts(uint32_t* counts, int reset) {
 }
 cudaError_t kv4_attention_counts(uint32_t* counts, int reset);  // ps_kv4_attention.cu
 
+// SMs of the current device (of a B200 where there is none).
+static inline int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess &&
+      n > 0)
+    return n;
+  return 148;
+}
+
 // A cache as kernels see it.
 struct Kv4Dev {
   unsigned char* pages;

@@ -1411,14 +1411,6 @@ struct APlan {
   int64_t ws_bytes;
 };
 
-static int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess &&
-      n > 0)
-    return n;
-  return 148;
-}
-
 // Key chunks per unit: the least modelled time, in tile times of one CTA.  `slots` CTAs run at once; a
 // CTA takes about three tile times to start and finish; partial results cost a second launch.
 static int choose_chunks(int64_t units, int tiles, int64_t slots) {

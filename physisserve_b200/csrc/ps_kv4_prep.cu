@@ -538,7 +538,8 @@ static void choose_split(int heads, int max_nb, int* nb, int* warps) {
   }
 }
 
-static int build_prep(const ps_kv4_prep_args* a, PPlan* plan) {
+// `sms`: of the device that the launch is for (its work split alone depends on it).
+static int build_prep(const ps_kv4_prep_args* a, int sms, PPlan* plan) {
   clear_error();
   if (!a) return fail(PS_ERR_NULL, "args is NULL");
   if (a->dtype != PS_BF16 && a->dtype != PS_F32) return fail(PS_ERR_DTYPE, "dtype %d is not PS_BF16 or PS_F32", a->dtype);
@@ -681,15 +682,16 @@ static int build_prep(const ps_kv4_prep_args* a, PPlan* plan) {
   plan->dtype = a->dtype;
   int warps = 1;
   plan->nb = 1;
-  // A launch whose tokens are all resident at once (18 warps an SM) is bound by the time of a token, not by
-  // throughput: then one block a thread, or two of bf16, whichever come to fit first.  8 tokens of 12 heads 3.2 us
-  // against 5.7, 800 tokens 6.0 against 7.5, 400 tokens of 40 heads 7.7 against 10.7; past it 1 560 tokens of 12
-  // heads 10.4 (one block) against 8.6.
+  // A launch whose tokens are all resident at once (18 warps an SM, at the 112 registers of two blocks a thread) is
+  // bound by the time of a token, not by throughput: then one block a thread, or two of bf16, whichever come to fit
+  // first.  8 tokens of 12 heads 3.2 us against 5.7, 800 tokens 6.0 against 7.5, 400 tokens of 40 heads 7.7 against
+  // 10.7; past it 1 560 tokens of 12 heads 10.4 (one block) against 8.6.
   const int most = a->heads > hk ? a->heads : hk;
   choose_split(most, max_blocks(a->dtype), &plan->nb, &warps);
+  const int64_t resident = 18ll * sms;
   for (int n = a->dtype == PS_BF16 ? 2 : 1; n >= 1; --n) {
     const int w = (most + 4 * n - 1) / (4 * n);
-    if (n < plan->nb && w * 32 <= kMaxTpt && total * w <= 148 * 18) {
+    if (n < plan->nb && w * 32 <= kMaxTpt && total * w <= resident) {
       plan->nb = n;
       warps = w;
     }
@@ -810,12 +812,12 @@ int kv4_check_cache(const ps_kv4_cache& c, Kv4Dev* d, int64_t* rows) {
 
 extern "C" int32_t ps_kv4_prep_validate(const ps_kv4_prep_args* args) {
   ps::PPlan plan;
-  return ps::build_prep(args, &plan);
+  return ps::build_prep(args, 148, &plan);
 }
 
 extern "C" int32_t ps_qk_norm_rope_kv4(const ps_kv4_prep_args* args, void* stream) {
   ps::PPlan plan;
-  const int rc = ps::build_prep(args, &plan);
+  const int rc = ps::build_prep(args, ps::sm_count(), &plan);
   if (rc != PS_OK || plan.blocks == 0) return rc;
   const bool full = plan.params.flags == ps::kFull;
   auto fn = ps::prep_fn(plan.dtype, plan.nb, full);
