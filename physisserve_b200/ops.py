@@ -936,7 +936,7 @@ def read_kv4(pages: torch.Tensor, table: torch.Tensor, tokens: int, *, row0: int
             continue
         if t.dtype is not dtype or t.get_device() != device_index:
             raise PrepError(f"{name} is {t.dtype} on {t.device}, expected {dtype} on {pages.device}")
-        if t.shape[0] != members or t.shape[1] != tokens:
+        if t.shape[:2] != (members, tokens):
             raise PrepError(f"{name} must be [{members}, {tokens}, {C}], got {tuple(t.shape)}")
         outs.append(t)
         strides.append(_member_rows(t, C, name))

@@ -993,3 +993,12 @@ def test_append_to_a_ring_of_nearly_two_to_the_31_frames():
     at = torch.cat([torch.tensor([1, 1]) * page_rows + torch.tensor([125, 126]), 2 * page_rows + torch.arange(3)])
     kv4.store(want, torch.arange(3)[None], at, x.view(5, heads, 128), 1, 1.0)
     assert torch.equal(pages.cpu(), want)
+
+
+def test_read_refuses_outputs_of_other_shapes():
+    pages, table, _, _ = fill(2, 20, 1, 16, 71)
+    dev = pages.to(DEV), table.to(DEV)
+    for shape in ((2,), (), (2, 19, 128), (1, 20, 128), (2, 20, 64), (2, 20)):
+        for name in ("k_out", "v_out"):
+            with pytest.raises(ops.PrepError, match=name):
+                ops.read_kv4(*dev, 20, **{name: torch.empty(shape, dtype=torch.bfloat16, device=DEV)})
