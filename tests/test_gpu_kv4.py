@@ -1002,3 +1002,21 @@ def test_read_refuses_outputs_of_other_shapes():
         for name in ("k_out", "v_out"):
             with pytest.raises(ops.PrepError, match=name):
                 ops.read_kv4(*dev, 20, **{name: torch.empty(shape, dtype=torch.bfloat16, device=DEV)})
+
+
+def test_tiles_offsets_beyond_32_bits():
+    """Many query rows over the last pages of a pool of over 4 GiB."""
+    heads, page_rows = 40, 128
+    n = (1 << 32) // (heads * 2 * page_rows * 72) + 5
+    pages = torch.zeros(n, heads, 2, page_rows * 72, dtype=torch.uint8, device=DEV)
+    _, _, k, v = fill(1, 300, heads, page_rows, 72, extra_pages=0)
+    at = torch.tensor([n - 1, 3, n - 2])
+    table = torch.arange(3, dtype=torch.int32)[None]
+    own = torch.full((3, heads, 2, page_rows * 72), 0xff, dtype=torch.uint8)
+    for which, x in ((0, k), (1, v)):
+        kv4.store(own, table, torch.arange(300), x[0].float(), which, 1.0)
+    pages[at.to(DEV)] = own.to(DEV)
+    k, v = (kv4.load(own, table, torch.arange(300), w, 1.0)[None] for w in (0, 1))
+    q = torch.randn(1, 130, heads * 128, generator=gen(73)).bfloat16()
+    got = ops.attention_kv4(q.to(DEV), pages, at[None].int().to(DEV), 300, heads=heads, kernel="tiles")
+    check_attention(got, q, k, v, [300], heads)
