@@ -26,8 +26,8 @@
  * element saturates, a NaN is stored as zero, and each such block is counted.
  *
  * A table entry outside [0, num_pages) is never followed: an append skips the
- * row, a read returns zeros, an attention leaves the page's keys out, and the
- * page is counted.  ps_kv4_counters reads both counts.
+ * row, a read returns zeros, an attention leaves the page's keys out, and each
+ * counts it in its own measure.  ps_kv4_counters reads both counts.
  *
  * Status codes, PS_API, ps_seq and the table modes come from physis_b200.h.
  * Every entry point validates on the host first, allocates nothing and is
@@ -133,7 +133,8 @@ typedef struct ps_kv4_attn_args {
   const void* q;  int64_t q_member_stride;   int64_t q_row_stride;   /* bf16 */
   void* out;      int64_t out_member_stride; int64_t out_row_stride; /* bf16 */
   const int32_t* kv_lens; /* device [members], or NULL */
-  void* workspace;        /* device scratch of ps_kv4_attention_workspace() bytes, 16-byte aligned */
+  void* workspace;        /* device scratch of ps_kv4_attention_workspace() bytes, 16-byte aligned;
+                           * calls that may run at once need one each */
   int64_t workspace_bytes;
   ps_kv4_cache cache;
 } ps_kv4_attn_args;
@@ -141,7 +142,8 @@ typedef struct ps_kv4_attn_args {
 /* RMSNorm(Q), RMSNorm(K), RoPE of Q and K, and the quantised write of rotated K
  * and of V: ps_qk_norm_rope_kv with the cache in the place of the ring.  Same
  * roundings; K's sum of squares is accumulated in 64 bits, so that the rows that
- * are quantised do not depend on the order of that sum. */
+ * are quantised do not depend on the order of that sum (but for one in some 2^28
+ * of those rows whose squares do not sum exactly in 64 bits). */
 PS_API int32_t ps_qk_norm_rope_kv4(const ps_kv4_prep_args* args, void* stream);
 PS_API int32_t ps_kv4_prep_validate(const ps_kv4_prep_args* args);
 

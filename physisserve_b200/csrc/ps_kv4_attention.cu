@@ -89,7 +89,7 @@ __device__ __forceinline__ float row_power(float top, float& back) {
 // rows kernel: up to 8 query rows of a K/V head
 // ---------------------------------------------------------------------------------------
 // Bound: HBM, 144 bytes a (key, K/V head); measured 16 members x 1 row of 12 heads over 34 320 keys in
-// 210 us, 70 % of the copy bandwidth: a 128-key tile takes an SM 0.62 us where HBM takes 0.42, and what
+// 209 to 225 us (on several B200s), 65 to 70 % of the copy bandwidth: a 128-key tile takes an SM 0.62 us where HBM takes 0.42, and what
 // takes it is the dequantising (ncu: 0.58 instructions a clock and scheduler, ALU 48 %, tensor pipe 23 %,
 // three CTAs' registers an SM).  One CTA takes a (member, K/V head, row block) and one chunk of its keys.  A producer warp brings 128-key tiles into a ring of shared-memory stages, one
 // bulk copy per page (K and V of a head lie together in a page); four warps take 32 keys of a tile
@@ -658,7 +658,7 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const __grid_constant_
 // ---------------------------------------------------------------------------------------
 // Bound: the tensor cores (4 * 128 * 256 flops a key), with the 16 exponentials a clock of an SM's
 // special-function unit next (256 of them a key: as many clocks as the products take).  Measured: 1 560
-// rows of 12 heads over 34 320 keys in 385 us, 854 TFLOP/s, half of the library's bf16 rate; a step of two
+// rows of 12 heads over 34 320 keys in 385 to 393 us, 840 to 854 TFLOP/s, half of the library's bf16 rate; a step of two
 // query tiles takes 4 350 clocks, the products 2 048 of them, the exponentials 2 275 when both tiles'
 // warps run them.  What is left is their waiting for one another.
 //

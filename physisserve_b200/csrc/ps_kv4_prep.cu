@@ -10,10 +10,12 @@
 //   bf16 ring.  Measured: 12 480 tokens of 40 heads in 150 us, 60 % of the copy bandwidth: about 7 400
 //   warp instructions a token at 0.6 a clock and scheduler are what the time goes to.
 //
-//   K's sum of squares is accumulated in fp64: bf16 squares are exact there and so is their sum, so
-//   the row's 1/sqrt -- and every rounding of what is quantised -- does not depend on the order of
-//   the sum.  (An fp32 sum's last bit moves one bf16 rounding in ~10^4 and with it now and then a
-//   4-bit code, a quarter of the value.)  A bf16 number becomes a double by moving its bits, not by
+//   K's sum of squares is accumulated in fp64: squares are exact there, and so is the sum of a bf16 row
+//   whose elements lie within about 2^11 of one another; of other rows, and of fp32 ones, the order
+//   moves the last of 53 bits, and with it a rounding of the row's 1/sqrt to 24 bits once in some 2^28
+//   rows.  So what is quantised does not depend on the order of the sum.  (An fp32 sum's last bit moves
+//   one bf16 rounding in ~10^4 and with it now and then a 4-bit code, a quarter of the value.)  A bf16
+//   number becomes a double by moving its bits, not by
 //   the conversion unit.  Q's sum stays fp32: nothing that it moves is quantised.
 //
 // kv4_read_kernel -- rows back as bf16 or fp32: a thread expands 8 code bytes and a scale of K and

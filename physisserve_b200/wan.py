@@ -309,7 +309,9 @@ class RingCache4:
 
     def reserve(self, rows: Sequence[int]) -> None:
         """Takes the pages that member b's first ``rows[b]`` rows still need (outside of a captured graph: the
-        new table entries are copied from the host; a graph's windows are reserved ahead of it)."""
+        new table entries are copied from the host; a graph's windows are reserved ahead of it).  The copy
+        waits for the stream, once for each call that needs pages: a cell whose whole window is reserved at
+        its start never waits again."""
         need = [-(-n // self.pool.page_rows) - len(held) for n, held in zip(rows, self._held)]
         count = sum(n for n in need if n > 0)
         if count == 0:
@@ -424,8 +426,8 @@ class RingAttention:
     faster than torch SDPA on the 1.3B and 14B block-call windows), with
     ``attention_kernel=False`` (or any other dtype / head size) through torch SDPA over the
     ring views, the reference's call.  Over a ``RingCache4`` it is ``ops.attention_kv4``, one call
-    whatever the members' window lengths (unlike ones are copied from the host: not in a captured
-    graph), or SDPA over the window read back.
+    whatever the members' window lengths (unlike ones are copied from the host, which waits for the
+    stream: not in a captured graph), or SDPA over the window read back.
     """
 
     def __init__(self, attention_kernel: bool = True):
