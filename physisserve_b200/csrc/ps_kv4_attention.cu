@@ -65,11 +65,15 @@ __device__ __forceinline__ int token_limit(const AParams& p, int n, int t) {
   return lim < 0 ? 0 : (lim > n ? n : static_cast<int>(lim));
 }
 
-// Probabilities are taken against a reference of their row that lags the running maximum by up to kLag (log2
-// units), so that it seldom moves, and 2^kLift times larger, so that fp16 holds them from 2^15 (its largest
-// power of two) down to 2^-24: what is lost of one is at most 2^-32 of the largest probability.  Without the
-// lift keys below 2^-25 of it were dropped from P V but not from the sum, all of them together.
-constexpr float kLag = 8.f, kLift = 7.f;
+// Probabilities are taken against a reference of their row, kLift (log2 units) below the largest score at the
+// time that it was set; it is set anew only when a score exceeds it by more than kTop, so that it seldom moves.
+// They reach 2^kTop then, and fp16 holds them from there (2^15 is its largest power of two) down to 2^-24: what is
+// lost of one is at most 2^-32 of the largest probability.  With no lift keys below 2^-25 of it were dropped from
+// P V but not from the sum, all of them together.  Both roundings are directed, so that kTop holds for scores
+// whose steps are larger than 1 too.
+constexpr float kLift = 7.f, kTop = 15.f;
+__device__ __forceinline__ float reference_of(float top) { return __fadd_ru(top, -kLift); }
+__device__ __forceinline__ float most_of(float reference) { return __fadd_rd(reference, kTop); }
 
 // Power of two that brings a row's largest magnitude `top` (>= 0) into [1, 2), and its inverse; 1 for
 // zero, subnormal and non-finite rows.  The inverse of 2^127 is subnormal: rows from there on come into
@@ -440,11 +444,13 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
         }
       }
       bool grow = false;
+      {
+        const float most[2] = {most_of(m[0]), most_of(m[1])};
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) grow |= acc[u][e] > m[e & 1] + kLag;
-      // The reference of a row moves only when a score exceeds it by more than kLag.
+          for (int e = 0; e < 4; ++e) grow |= acc[u][e] > most[e & 1];
+      }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -454,7 +460,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          const float next = fmaxf(m[e], top);
+          const float next = fmaxf(m[e], reference_of(top));
           const float alpha = next == -INFINITY ? 1.f : fast_exp2(m[e] - next);
           m[e] = next;
           l[e] *= alpha;
@@ -467,7 +473,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) kv4_rows_kernel(const __grid_c
       }
       uint32_t pb[U][2];
       {
-        const float r0 = m[0] == -INFINITY ? 0.f : m[0] - kLift, r1 = m[1] == -INFINITY ? 0.f : m[1] - kLift;
+        const float r0 = m[0] == -INFINITY ? 0.f : m[0], r1 = m[1] == -INFINITY ? 0.f : m[1];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const float p0 = fast_exp2(acc[u][0] - r0), p1 = fast_exp2(acc[u][1] - r1);
@@ -1247,12 +1253,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
           largest(xb);
         }
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
-        // The reference moves only when a score exceeds it by more than kLag.
-        const bool grow = top > m + kLag;
-        const float alpha = grow ? fast_exp2(m - top) : 1.f;
+        const bool grow = top > most_of(m);
+        const float next = grow ? reference_of(top) : m;
+        const float alpha = grow ? fast_exp2(m - next) : 1.f;
         if (grow) {
           l *= alpha;
-          m = top;
+          m = next;
         }
         // O holds this segment's earlier tiles (their P V have completed: S was committed after them).
         if (__any_sync(0xffffffffu, grow) && j > w.j0) {
@@ -1266,7 +1272,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
             tmem_st16(o_addr + 16 * c, o);
           }
         }
-        const float ref = m == -INFINITY ? 0.f : m - kLift;
+        const float ref = m == -INFINITY ? 0.f : m;
         const f32x2 scale2 = f2_make(scale, scale), ref2 = f2_make(-ref, -ref);
         f32x2 sum[2] = {0, 0};
         // Tile 0's k-th turn follows tile 1's (k-1)-th, tile 1's k-th follows tile 0's k-th.

@@ -1020,3 +1020,44 @@ def test_tiles_offsets_beyond_32_bits():
     q = torch.randn(1, 130, heads * 128, generator=gen(73)).bfloat16()
     got = ops.attention_kv4(q.to(DEV), pages, at[None].int().to(DEV), 300, heads=heads, kernel="tiles")
     check_attention(got, q, k, v, [300], heads)
+
+
+# ---------------------------------------------------------------------------------------
+# Scores far beyond the range of the exponentials
+# ---------------------------------------------------------------------------------------
+def one_element_cache(rows, elements, seed):
+    """A cache of one head whose keys are zero but for the given {element: e2m1 numbers}, under scales of 1."""
+    n, table = make_table(1, -(-rows // 128), 1, seed)
+    pages = torch.full((n, 1, 2, 128 * 72), 0xff, dtype=torch.uint8)
+    kv4.store(pages, table, torch.arange(rows), torch.rand(rows, 1, 128, generator=gen(seed)) + 0.5, 1, 1.0)
+    nibbles, x = torch.zeros(rows, 128, dtype=torch.uint8), torch.zeros(rows, 128)
+    for e, numbers in elements.items():
+        x[:, e] = numbers
+        nibbles[:, e] = torch.searchsorted(kv4.E2M1, numbers.abs().double()).byte() | (torch.signbit(numbers).byte() << 3)
+    codes, scales = kv4.split(pages)
+    page, row = kv4.place(table, torch.arange(rows), 128)
+    codes[page, 0, 0, row], scales[page, 0, 0, row] = nibbles[:, 0::2] | (nibbles[:, 1::2] << 4), 0x38
+    k, v = (kv4.load(pages, table, torch.arange(rows), w, 1.0)[None] for w in (0, 1))
+    assert torch.equal(k[0, :, 0].float(), x)
+    return pages, table, k, v
+
+
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
+@pytest.mark.parametrize("exponent", [10, 20, 24, 25])
+@pytest.mark.parametrize("step", [1, 2, 4, 8])
+def test_attention_of_scores_a_few_steps_apart(step, exponent, kernel):
+    """Scores in log2 units of 2^exponent and a little more, exact in fp32 (up to 2^25 in steps of 4): the
+    reference lags behind them, and its distance is rounded like they are."""
+    if exponent == 25 and step < 4 or exponent == 24 and step < 2:
+        step *= 4
+    rows, Lq = 600, 4
+    more = torch.zeros(rows)
+    more[[130, 260]] = 1.0                # behind the first tile
+    more[[391, 500]] = 2.0
+    pages, table, k, v = one_element_cache(rows, {0: torch.full((rows,), 4.0), 64: more}, 82)
+    q = torch.zeros(1, Lq, 128, dtype=torch.bfloat16)
+    q[0, :, 0], q[0, :, 64] = 2.0 ** (exponent - 2), float(step)
+    q[0, 1::2, 0] *= -1.0
+    scale = 0.6931471805599453            # times log2(e): 1
+    got = ops.attention_kv4(q.to(DEV), pages.to(DEV), table.to(DEV), rows, heads=1, scale=scale, key_chunks=1, kernel=kernel)
+    check_attention(got, q, k, v, [rows], 1, scale=scale)
