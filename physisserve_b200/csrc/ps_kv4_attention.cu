@@ -664,7 +664,7 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const __grid_constant_
 // ---------------------------------------------------------------------------------------
 // Bound: the tensor cores (4 * 128 * 256 flops a key), with the 16 exponentials a clock of an SM's
 // special-function unit next (256 of them a key: as many clocks as the products take).  Measured: 1 560
-// rows of 12 heads over 34 320 keys in 385 to 393 us, 840 to 854 TFLOP/s, half of the library's bf16 rate; a step of two
+// rows of 12 heads over 34 320 keys in 388 to 396 us, 830 to 848 TFLOP/s, half of the library's bf16 rate; a step of two
 // query tiles takes 4 350 clocks, the products 2 048 of them, the exponentials 2 275 when both tiles'
 // warps run them.  What is left is their waiting for one another.
 //
@@ -712,8 +712,15 @@ enum TBar {
 };
 constexpr int kOffTmem = kOffBars + 8 * kTBars, kOffAbort = kOffTmem + 4, kOffThere = kOffAbort + 4;
 constexpr int kOffStart = (kOffThere + 4 * kRawSlots + 15) & ~15;
-constexpr int kTilesSmem = kOffStart + 32 + 1024;
+constexpr int kOffFactor = kOffStart + 32;  // [256] the factor of a row's scores in tensor memory
+constexpr int kTilesSmem = kOffFactor + 4 * kUnitRows + 1024;
 static_assert(kTilesSmem <= 227 * 1024, "tiles exceed shared memory");
+// The softmax fuses a score's scaling with the taking off of its row's reference.  The reference is made of scores
+// scaled and rounded, and from 2^24 on the product that is not rounded may lie further from it than fp16's range
+// above kTop has room for.  A row whose reference gets beyond kNear has its scores scaled, and so rounded, in
+// tensor memory from then on.  (Rounding every product in the softmax itself: 1.3B block call 385 -> 392 us; this
+// costs 391 -> 392.5.)
+constexpr float kNear = 0x1p22f;
 __host__ __device__ constexpr int col_o(int i) { return 256 * i; }
 __host__ __device__ constexpr int col_s(int i) { return 256 * i + 128; }
 // kind::f16 with fp16 operands, fp32 accumulators, M = N = 128; b_mn: B's N runs along its rows.
@@ -771,6 +778,20 @@ __device__ __forceinline__ bool spin_bar(uint32_t bar, uint32_t parity, volatile
 }
 __device__ __forceinline__ bool warp_spin(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   return __all_sync(0xffffffffu, spin_bar(bar, parity, abort_flag));
+}
+
+// The scores of this thread's TMEM lane times f.
+__device__ __noinline__ void scale_scores(uint32_t s_addr, float f) {
+#pragma unroll 1
+  for (int col = 0; col < 128; col += 16) {
+    uint32_t y[16];
+    tmem_ld16(s_addr + col, y);
+    tmem_wait_ld16(y);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+    tmem_st16(s_addr + col, y);
+  }
+  tmem_wait_st();
 }
 
 // Steps of a unit of member b with n window rows: the 128-key tiles that any of its rows sees, at least
@@ -1171,6 +1192,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
       // does not see every key.
       const int j_mask = token_limit(p, n, min(w.qb * kUnitRows + qi * kM, p.rows - 1) / p.group) / kTileKeys;
       float scale;
+      float* const factor = reinterpret_cast<float*>(smem + kOffFactor) + qi * kM + row;
+      *factor = 1.f;
       {
         // Q, scaled to fp16 and stored 128-byte swizzled.
         uint4 x[16];
@@ -1209,15 +1232,17 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
         return __ballot_sync(0xffffffffu, bad);
       };
       const int pages_seen = (w.lim_top + (1 << shift) - 1) >> shift;
-      const bool any_bad = bad_pages(w.j0 * segs_tile, min(w.j1 * segs_tile, pages_seen)) != 0;
+      // Bit 0: a page that is not there; bit 1: a row of the warp whose scores are scaled in tensor memory.
+      int careful = bad_pages(w.j0 * segs_tile, min(w.j1 * segs_tile, pages_seen)) != 0 ? 1 : 0;
       float m = -INFINITY, l = 0.f;
       for (int j = w.j0; j < w.j1; ++j, ++n_tiles) {
         if (!(ok = warp_spin(bar(kSFull + qi), n_tiles & 1, abort_flag))) break;
         tc_fence_after();
         // A tile of which the row does not see every key: -inf over the others, in tensor memory, so that
-        // the passes below need not know.
-        if (j >= j_mask || any_bad) {
-          const uint32_t bad = any_bad ? bad_pages(j * segs_tile, min((j + 1) * segs_tile, pages_seen)) : 0;
+        // the passes below need not know; nor of scores that are scaled here.
+        if (j >= j_mask || careful) {
+          if (__builtin_expect(careful & 2, 0)) scale_scores(s_addr, *factor);
+          const uint32_t bad = careful & 1 ? bad_pages(j * segs_tile, min((j + 1) * segs_tile, pages_seen)) : 0;
           const int valid = lim - j * kTileKeys;
 #pragma unroll 1
           for (int col = 0; col < 128; col += 16) {
@@ -1260,16 +1285,29 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
           l *= alpha;
           m = next;
         }
-        // O holds this segment's earlier tiles (their P V have completed: S was committed after them).
-        if (__any_sync(0xffffffffu, grow) && j > w.j0) {
+        if (__any_sync(0xffffffffu, grow)) {
+          // O holds this segment's earlier tiles (their P V have completed: S was committed after them).
+          if (j > w.j0) {
 #pragma unroll 1
-          for (int c = 0; c < 8; ++c) {
-            uint32_t o[16];
-            tmem_ld16(o_addr + 16 * c, o);
-            tmem_wait_ld16(o);
+            for (int c = 0; c < 8; ++c) {
+              uint32_t o[16];
+              tmem_ld16(o_addr + 16 * c, o);
+              tmem_wait_ld16(o);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-            tmem_st16(o_addr + 16 * c, o);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st16(o_addr + 16 * c, o);
+            }
+          }
+          const bool far = grow && !(fabsf(m) < kNear) && scale != 1.f;  // (once: its scale is 1 then)
+          if (__builtin_expect(__any_sync(0xffffffffu, far), 0)) {
+            careful |= 2;
+            tmem_wait_ld32(xa);
+            scale_scores(s_addr, far ? scale : 1.f);
+            tmem_ld32(s_addr, xa);
+            if (far) {
+              *factor = scale;
+              scale = 1.f;
+            }
           }
         }
         const float ref = m == -INFINITY ? 0.f : m;

@@ -1061,3 +1061,20 @@ def test_attention_of_scores_a_few_steps_apart(step, exponent, kernel):
     scale = 0.6931471805599453            # times log2(e): 1
     got = ops.attention_kv4(q.to(DEV), pages.to(DEV), table.to(DEV), rows, heads=1, scale=scale, key_chunks=1, kernel=kernel)
     check_attention(got, q, k, v, [rows], 1, scale=scale)
+
+
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
+@pytest.mark.parametrize("Lq", [3, 200])
+@pytest.mark.parametrize("exponent", [10, 21, 24, 25, 26, 28, 34, 60, 100])
+def test_attention_of_scores_of_any_size(exponent, Lq, kernel):
+    """Scores of about 2^exponent, of either sign, a few keys sharing the largest: their V's mean."""
+    rows = 700
+    numbers = torch.tensor([0.5, 1.0, 2.0, 3.0])[torch.randint(0, 4, (rows,), generator=gen(80))]
+    numbers[::90] = 4.0
+    numbers[::70] = -4.0
+    pages, table, k, v = one_element_cache(rows, {0: numbers}, 81)
+    q = torch.zeros(1, Lq, 128, dtype=torch.bfloat16)
+    q[0, :, 0] = torch.tensor([1.0, -1.25, 1.40625, 1.9921875]).repeat(-(-Lq // 4))[:Lq] * 2.0 ** exponent
+    for chunks in (1, 0):
+        got = ops.attention_kv4(q.to(DEV), pages.to(DEV), table.to(DEV), rows, heads=1, key_chunks=chunks, kernel=kernel)
+        check_attention(got, q, k, v, [rows], 1)
