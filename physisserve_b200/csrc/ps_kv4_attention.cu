@@ -92,12 +92,13 @@ __device__ __forceinline__ float row_power(float top, float& back) {
 // ---------------------------------------------------------------------------------------
 // rows kernel: up to 8 query rows of a K/V head
 // ---------------------------------------------------------------------------------------
-// Bound: HBM, 144 bytes a (key, K/V head); measured 16 members x 1 row of 12 heads over 34 320 keys in
-// 209 to 225 us (on several B200s), 65 to 70 % of the copy bandwidth: a 128-key tile takes an SM 0.62 us where HBM takes 0.42, and what
-// takes it is the dequantising (ncu: 0.58 instructions a clock and scheduler, ALU 48 %, tensor pipe 23 %,
-// three CTAs' registers an SM).  One CTA takes a (member, K/V head, row block) and one chunk of its keys.  A producer warp brings 128-key tiles into a ring of shared-memory stages, one
-// bulk copy per page (K and V of a head lie together in a page); four warps take 32 keys of a tile
-// each.  Both products run transposed on mma.m16n8k16 -- S^T = K Q^T and O^T = V^T P^T -- so that the
+// Bound: HBM, 144 bytes a (key, K/V head); measured 16 members x 1 row of 12 heads over 34 320 keys in 209
+// to 225 us (on several B200s), 65 to 70 % of the copy bandwidth: a 128-key tile takes an SM 0.62 us where
+// HBM takes 0.42, and what takes it is the dequantising (ncu: 0.58 instructions a clock and scheduler, ALU
+// 48 %, tensor pipe 23 %, three CTAs' registers an SM).  One CTA takes a (member, K/V head, row block) and
+// one chunk of its keys.  A producer warp brings 128-key tiles into a ring of shared-memory stages, one
+// bulk copy per page (K and V of a head lie together in a page); four warps take 32 keys of a tile each.
+// Both products run transposed on mma.m16n8k16 -- S^T = K Q^T and O^T = V^T P^T -- so that the
 // keys and the head dimension fill the 16-row side and eight query rows the 8-column side: a single
 // query row wastes 7/8 of an otherwise idle tensor pipe and no memory traffic, and a fragment of K or
 // V is dequantised once whatever the number of rows.

@@ -968,7 +968,8 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, kv_
     before it.  A row that sees nothing gets zeros.  Returns ``out`` [B, Lq, heads*128] (allocated if
     not given).  ``kernel`` ("auto", "rows", "tiles") and ``key_chunks`` override the kernel and the rows
     kernel's work split; ``workspace`` is a contiguous tensor on a 16-byte boundary for the partial results of key
-    chunks (allocated if None or too small).  ``check_timeouts=True`` synchronises and raises ``PrepError`` if a bounded wait ran out.
+    chunks (allocated if None or too small).  ``check_timeouts=True`` synchronises and raises ``PrepError`` if a
+    bounded wait ran out.
     """
     device_index, members, page_rows, cache = _kv4_cache(pages, table, k_scale, v_scale)
     if q.dtype is not torch.bfloat16:

@@ -236,6 +236,12 @@ class Kv4Pool:
         self._taken: set[int] = set()
         self._lock = threading.Lock()
 
+    def __getstate__(self):
+        return {name: value for name, value in self.__dict__.items() if name != "_lock"}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state, _lock=threading.Lock())
+
     @property
     def free_pages(self) -> int:
         return len(self._free)

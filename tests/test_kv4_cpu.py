@@ -369,3 +369,16 @@ def test_a_reservation_is_taken_whole_or_not_at_all():
     with pytest.raises(ops.PrepError, match="free pages"):
         cell.reserve([40, 17])
     assert pool.free_pages == 3 and bool((cell.table == -1).all()) and cell._held == [[], []]
+
+
+def test_a_cache_is_copied_with_its_pool():
+    import copy
+
+    from physisserve_b200.wan import RingCache4
+
+    cell = RingCache4(heads=1, grid_h=2, grid_w=4, capacity=4, sink_frames=2, batch=1, page_rows=16)
+    cell.reserve([20])
+    other = copy.deepcopy(cell)
+    other.reserve([40])
+    assert cell.pool.free_pages == other.pool.free_pages + 1
+    assert torch.equal(cell.table[0, :2], other.table[0, :2]) and cell._held != other._held
